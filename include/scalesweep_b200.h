@@ -301,6 +301,109 @@ int ssw_global_scale_inv_noalloc(const void* input, int input_dtype, int64_t num
                                  float fp8_max, float* input_scale_out, float* amax_out,
                                  void* stream);
 
+/*
+ * NVFP4 KV cache.  A page holds page_size tokens of every kv head:
+ *   codes  [num_pages, 2, kv_heads, page_size, head_size / 2]   (E2M1, element 2j in the low nibble)
+ *   scales [num_pages, 2, kv_heads, page_size, head_size / 16]  (E4M3, one per 16 elements)
+ * where index 0 of the second axis holds keys, index 1 values.  Pages lie
+ * codes_page_stride / scales_page_stride bytes apart (multiples of 16); inside
+ * a page everything is contiguous.  input_scale: two floats on the device, the
+ * multipliers of the keys and of the values; a stored value stands for
+ * code * scale / multiplier.  No counterpart in the reference, whose
+ * quantizer stops at the linear layers' activations.
+ */
+typedef struct {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t codes_page_stride;
+  int64_t scales_page_stride;
+  const float* input_scale;
+  int64_t num_pages;
+  int32_t page_size; /* 16, 32, 64 or 128 */
+  int32_t kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+} ssw_kv_cache;
+
+/* A [tokens, heads, head_size] tensor of 16-bit floats, 16-byte aligned; the
+ * strides are in elements, multiples of 8; the last dimension is contiguous. */
+typedef struct {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} ssw_kv_heads;
+
+/*
+ * Rotary positions on query and key, and the scalesweep_mse quantization of
+ * the rotated keys and the values into the cache's rows slot_mapping[t] =
+ * page * page_size + row (distinct; a negative slot, or one past the last
+ * page, is not written).  cos_sin_cache: float [max_position, rotary_dim], the
+ * cosines then the sines of a position.  is_neox: pairs (i, i + rotary_dim/2),
+ * else (2i, 2i + 1); elements past rotary_dim (a multiple of 16) are left.
+ * query_out receives the rotated query (it may be query); key and value are
+ * only read.  A position outside the table gives a query of NaN and writes no
+ * row.  query_out must not overlap key or value.
+ * The bytes equal ssw_scalesweep_mse_nvfp4_quant_out's on the rotated keys,
+ * rounded to their type, and the values.
+ */
+int ssw_rotary_scalesweep_mse_nvfp4_kv_write(const ssw_kv_cache* cache, int dtype, int64_t tokens,
+                                             int q_heads, const ssw_kv_heads* query,
+                                             const ssw_kv_heads* key, const ssw_kv_heads* value,
+                                             const ssw_kv_heads* query_out,
+                                             const int64_t* positions, const float* cos_sin_cache,
+                                             int64_t max_position, int rotary_dim, int is_neox,
+                                             const int64_t* slot_mapping, void* stream);
+
+/*
+ * The values at slot_mapping as 16-bit floats, key and value [tokens,
+ * kv_heads, head_size] contiguous: code * scale / multiplier, the quotient
+ * rounded to binary32 and then to the type; zeros for a slot outside the cache.
+ */
+int ssw_nvfp4_kv_gather(const ssw_kv_cache* cache, int dtype, int64_t tokens,
+                        const int64_t* slot_mapping, void* key, void* value, void* stream);
+
+/*
+ * Attention of a batch of sequences over the cache.  Sequence b has the query
+ * rows query_start[b] .. query_start[b+1] - 1 and seq_lens[b] keys, its new
+ * tokens' included: key j lies in page block_table[b][j / page_size] at row
+ * j % page_size.  An entry outside 0 .. num_pages - 1 holds no keys (pages
+ * that a window has left behind).  Query i of a sequence has the position
+ * seq_lens[b] - (its query rows) + i; causal: it sees the keys up to that
+ * position; window >= 0: only those from position - window on.  A row that
+ * sees no key gives zeros and a log-sum-exp of -inf.  Rows of out and lse that
+ * belong to no sequence are left as they were.
+ * out[r] = sum_j softmax_j(softmax_scale * q[r] . K[j]) V[j]; query head h uses
+ * kv head h / (q_heads / kv_heads).  lse (may be null): float [tokens,
+ * q_heads], the natural log of the sum of exp(softmax_scale * q . K).
+ * max_query_len and max_seq_len bound the batch's lengths from above.
+ * status (may be null): an int set to 1 if a bounded device-side wait gave up
+ * (the output is then undefined).
+ */
+typedef struct {
+  const int32_t* block_table;
+  int64_t block_table_stride; /* elements between sequences */
+  const int32_t* seq_lens;
+  const int32_t* query_start;
+  float* lse;
+  int32_t* status;
+  int64_t tokens; /* rows of query and out */
+  int32_t seqs;
+  int32_t block_table_columns;
+  int32_t q_heads;
+  int32_t max_query_len;
+  int32_t max_seq_len;
+  int32_t causal;
+  int32_t window; /* < 0: none */
+  float softmax_scale;
+} ssw_kv_attention;
+
+/* Workspace of the call below (0: none needed), 16-byte aligned; -1 for
+ * arguments that the call refuses.  Two calls that may overlap need two. */
+int64_t ssw_nvfp4_paged_attention_workspace_bytes(const ssw_kv_cache* cache,
+                                                  const ssw_kv_attention* args, int dtype);
+int ssw_nvfp4_paged_attention(const ssw_kv_cache* cache, const ssw_kv_attention* args, int dtype,
+                              const ssw_kv_heads* query, const ssw_kv_heads* out, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

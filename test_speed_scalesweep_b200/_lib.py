@@ -49,7 +49,36 @@ _SIGNATURES = {
     "ssw_nvfp4_mma_rate_probe": (_int, [_int, _int, _c_p, _c_p, _c_p]),
     "ssw_global_scale_inv_noalloc_max_numel": (_i64, []),
     "ssw_global_scale_inv_noalloc": (_int, [_c_p, _int, _i64, _f32, _c_p, _c_p, _c_p]),
+    "ssw_rotary_scalesweep_mse_nvfp4_kv_write": (_int, [_c_p, _int, _i64, _int, _c_p, _c_p, _c_p, _c_p,
+                                                        _c_p, _c_p, _i64, _int, _int, _c_p, _c_p]),
+    "ssw_nvfp4_kv_gather": (_int, [_c_p, _int, _i64, _c_p, _c_p, _c_p, _c_p]),
+    "ssw_nvfp4_paged_attention_workspace_bytes": (_i64, [_c_p, _c_p, _int]),
+    "ssw_nvfp4_paged_attention": (_int, [_c_p, _c_p, _int, _c_p, _c_p, _c_p, _i64, _c_p]),
 }
+
+
+class KVCache(ctypes.Structure):
+    """``ssw_kv_cache``."""
+    _fields_ = [("codes", _c_p), ("scales", _c_p), ("codes_page_stride", _i64),
+                ("scales_page_stride", _i64), ("input_scale", _c_p), ("num_pages", _i64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_size", ctypes.c_int32)]
+
+
+class KVHeads(ctypes.Structure):
+    """``ssw_kv_heads``."""
+    _fields_ = [("data", _c_p), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+class KVAttention(ctypes.Structure):
+    """``ssw_kv_attention``."""
+    _fields_ = [("block_table", _c_p), ("block_table_stride", _i64), ("seq_lens", _c_p),
+                ("query_start", _c_p), ("lse", _c_p), ("status", _c_p), ("tokens", _i64),
+                ("seqs", ctypes.c_int32), ("block_table_columns", ctypes.c_int32),
+                ("q_heads", ctypes.c_int32), ("max_query_len", ctypes.c_int32),
+                ("max_seq_len", ctypes.c_int32), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("softmax_scale", _f32)]
+
 
 ABI_VERSION = 1
 SSW_OK, SSW_ERR_INVALID_ARGUMENT, SSW_ERR_UNSUPPORTED, SSW_ERR_CUDA, SSW_ERR_TIMEOUT = range(5)
@@ -111,3 +140,21 @@ def dtype_code(t: torch.Tensor) -> int:
 
 def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Nothing:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, at no cost where it is the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(device)

@@ -1,0 +1,83 @@
+// Internal launch interface of the NVFP4 KV-cache kernels (not part of the C ABI).
+//
+// A cache page holds `page_size` tokens of every kv head:
+//   codes  [pages, 2 (key, value), kv_heads, page_size, head_size / 2]   E2M1, element 2j in the low nibble
+//   scales [pages, 2 (key, value), kv_heads, page_size, head_size / 16]  E4M3, one per 16 elements
+// The pages may lie any multiple of 16 bytes apart (a layer of a cache that
+// holds all layers); inside a page everything is contiguous.  A value is
+// code * scale / multiplier, the multiplier being one float each for the keys
+// and the values of a layer.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace ssw {
+namespace kv {
+
+struct Cache {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t codes_page_stride;   // bytes
+  int64_t scales_page_stride;  // bytes
+  const float* multiplier;     // [2]: keys, values
+  int64_t num_pages;
+  int32_t page_size;           // 16, 32, 64 or 128
+  int32_t kv_heads;
+  int32_t head_size;           // 64, 128 or 256
+};
+
+// A [tokens, heads, head_size] tensor of 16-bit floats: strides in elements,
+// multiples of 8; the last dimension is contiguous.
+struct Heads {
+  uint16_t* p;
+  int64_t token_stride;
+  int64_t head_stride;
+};
+
+struct WriteArgs {
+  Cache cache;
+  Heads q, k, v, q_out;
+  const int64_t* positions;  // [tokens]
+  const float* cos_sin;      // [max_position, rotary_dim]: cos, then sin
+  int64_t max_position;
+  const int64_t* slots;      // [tokens]: page * page_size + row, < 0 = padding
+  int64_t tokens;
+  int32_t q_heads;
+  int32_t rotary_dim;        // a multiple of 16, <= head_size
+  int32_t neox;              // 1: pairs (i, i + rotary_dim / 2); 0: pairs (2i, 2i + 1)
+  int32_t dtype;             // kDTypeBF16 / kDTypeF16
+};
+cudaError_t launch_write(const WriteArgs& a, int device_sms, cudaStream_t stream);
+
+struct GatherArgs {
+  Cache cache;
+  const int64_t* slots;  // [tokens]
+  int64_t tokens;
+  uint16_t* key;         // [tokens, kv_heads, head_size]
+  uint16_t* value;
+  int32_t dtype;
+};
+cudaError_t launch_gather(const GatherArgs& a, int device_sms, cudaStream_t stream);
+
+struct AttendArgs {
+  Cache cache;
+  Heads q, out;
+  const int32_t* block_table;  // [seqs, table_columns] of page ids
+  int64_t table_stride;        // elements
+  const int32_t* seq_lens;     // [seqs]: keys of a sequence, its new tokens' included
+  const int32_t* query_start;  // [seqs + 1]: first query token of a sequence
+  float* lse;                  // [tokens, q_heads] or null
+  float* workspace;            // partial results of split sequences
+  int32_t* status;             // or null
+  int64_t tokens;              // rows of q and out
+  int32_t seqs, table_columns, q_heads, max_query_len, max_seq_len;
+  int32_t causal, window;      // window < 0: none
+  int32_t dtype;
+  float softmax_scale;
+};
+int64_t attend_workspace_bytes(const AttendArgs& a, int device_sms);
+cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stream);
+
+}  // namespace kv
+}  // namespace ssw

@@ -1,0 +1,728 @@
+// Attention over an NVFP4 cache (layout in kv.cuh), one pass over its bytes:
+//
+//   O[r] = sum_j softmax_j(scale / mult_k * q[r] . K[j]) V[j] / mult_v
+//
+// for the query rows r of a sequence and the keys j that the causal order and
+// the window let r see; K and V are code * scale, which 16-bit floats (f16)
+// hold exactly (6 significant bits, 2^-10 .. 2688).
+//
+// All of a kv head's query heads share the dequantized keys, so the rows of a
+// tile are (token, head of the group) pairs, r = token * group + head.
+//
+// decode_kernel: tiles of 8, 16 or 32 rows, for single tokens and short
+// queries.  It is bound by the cache's bytes, so the products are laid out for
+// the cheapest dequantization, not for the tensor cores' rate: mma.sync with
+// the *cache* as its 16-row operand (S^T = K Q^T, O^T = V^T P^T) spends one
+// instruction per 256 cache elements however few rows the query has.
+//   - A contraction may visit its index in any order, so a thread's share of a
+//     key row is the contiguous quarter that one vector load gives, and Q is
+//     permuted to match; a thread needs the scales of its own quarter only.
+//   - For V the keys are contracted: two keys' codes are paired nibble by
+//     nibble (4 logic operations per 16 codes) and converted together.
+//   - Each warp takes every kWarps-th group of 32 keys of its CTA's share of
+//     the sequence with its own running maximum and sum, fetched by bulk copies
+//     into a ring of its own: no barrier between warps until the end.
+// Softmax statistics and both accumulators are binary32.  P is rounded to f16
+// (relative 2^-11, finer than a bf16 result) scaled by 2^kShift, so that
+// weights down to 2^-(14 + kShift) of the largest keep full precision.
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "kv.cuh"
+#include "quant.cuh"
+
+namespace ssw {
+namespace kv {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kKeys = 32;      // keys of a stage
+constexpr float kShift = 10.f;  // log2 of the scale of P
+constexpr float kSlack = 5.f;   // the maximum may grow by 2^kSlack before O is rescaled
+constexpr uint32_t kWaitLimit = 1u << 22;  // bounded spin
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+
+struct Params {
+  AttendArgs a;
+  int group;       // query heads of a kv head
+  int tiles;       // row tiles of the longest query
+  int splits;      // CTAs that share a tile's keys
+  int chunk;       // keys of a split, a multiple of kKeys * kWarps
+  int page_shift;
+  float* part_o;   // [split][row of q and head][head_size]
+  float* part_ml;  // [split][row of q and head][2]
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// Bounded wait for the phase with the given parity; false = gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two f16 from one byte of codes (element 0 in the low nibble).
+__device__ __forceinline__ uint32_t e2m1_h2(uint32_t word, int byte) {
+  uint32_t r;
+  const uint16_t b = (uint16_t)((word >> (8 * byte)) & 0xFF);
+  asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}"
+      : "=r"(r)
+      : "h"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_h2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The rows and keys of one tile.
+struct Tile {
+  int row0, rows;        // first of the sequence's rows, rows here
+  int first_token;       // global token of the sequence's token 0
+  int offset;            // position of the sequence's token 0
+  int beg, end;          // keys that any of its rows sees
+  int all_beg, all_end;  // keys that all of its rows see
+};
+
+__device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int tile_rows,
+                                        Tile& t) {
+  const AttendArgs& a = p.a;
+  const int q0 = a.query_start[seq];
+  int len = a.query_start[seq + 1] - q0;
+  if (q0 < 0 || len <= 0) return false;
+  const int kv = max(0, a.seq_lens[seq]);
+  t.offset = kv - len;
+  if (q0 >= a.tokens) return false;
+  if (len > a.tokens - q0) len = (int)(a.tokens - q0);
+  const int rows = len * p.group;
+  t.row0 = tile * tile_rows;
+  if (t.row0 >= rows) return false;
+  t.rows = min(tile_rows, rows - t.row0);
+  t.first_token = q0;
+  const int lo = t.offset + t.row0 / p.group;
+  const int hi = t.offset + (t.row0 + t.rows - 1) / p.group;
+  const int room = (int)min((int64_t)a.table_columns << p.page_shift, (int64_t)kv);
+  t.end = a.causal ? min(room, hi + 1) : room;
+  t.all_end = a.causal ? min(room, lo + 1) : room;
+  t.beg = a.window >= 0 ? max(0, lo - a.window) : 0;
+  t.all_beg = a.window >= 0 ? max(0, hi - a.window) : 0;
+  t.end = max(t.end, 0);
+  return true;
+}
+
+// Splits of a tile that hold keys (at least one, which then writes zeros).
+__device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
+  const int n = t.end - (t.beg & ~(kKeys - 1));
+  return max(1, (n + p.chunk - 1) / p.chunk);
+}
+
+template <int kD>
+struct Shape {
+  static constexpr int kCodeRow = kD / 2, kScaleRow = kD / 16;
+  static constexpr int kKCodes = kKeys * kCodeRow, kKScales = kKeys * kScaleRow;
+  static constexpr int kStage = 2 * (kKCodes + kKScales);
+  static constexpr int kStages = kD == 256 ? 2 : 4;
+  static constexpr int kRing = kStages * kStage;           // of a warp
+  static constexpr int kKSteps = kD / 16;
+};
+
+// Shared memory: the warps' rings, then their barriers.  The rings are reused
+// for the warps' partial results, kNT * 8 rows of kD + 2 floats each.
+template <int kD, int kNT>
+constexpr int smem_bytes() {
+  constexpr int ring = kWarps * Shape<kD>::kRing;
+  constexpr int merge = kWarps * kNT * 8 * (kD + 2) * 4;
+  return (ring > merge ? ring : merge) + kWarps * Shape<kD>::kStages * 8;
+}
+
+__device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype) {  // 2 values
+  if (dtype == kDTypeBF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+    *reinterpret_cast<__nv_bfloat162*>(dst) = h;
+  } else {
+    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(v[0], v[1]);
+  }
+}
+
+template <int kD, int kNT>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
+  using S = Shape<kD>;
+  constexpr int kRows = kNT * 8;
+  constexpr int kQuarter = kD / 4;             // elements of a key row per thread
+  constexpr int kKWords = kD / 32;             // 32-bit words of codes per thread and key row
+  constexpr int kVWords = kD / 64 < 1 ? 1 : kD / 64;  // words of codes per thread and value row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.y, head = blockIdx.z;
+  const int seq = blockIdx.x / p.tiles;
+  Tile tile;
+  if (!tile_of(p, seq, blockIdx.x % p.tiles, kRows, tile)) return;
+  const int base = tile.beg & ~(kKeys - 1);
+  if (split > 0 && base + (int64_t)split * p.chunk >= tile.end) return;
+  const int c0 = base + split * p.chunk;
+  const int c1 = min((int64_t)tile.end, (int64_t)c0 + p.chunk);
+
+  constexpr int kBarOff = smem_bytes<kD, kNT>() - kWarps * S::kStages * 8;
+  const uint32_t ring = smem_u32(smem) + warp * S::kRing;
+  const uint32_t bars = smem_u32(smem) + kBarOff + warp * S::kStages * 8;
+  if (lane == 0) {
+    for (int s = 0; s < S::kStages; ++s) mbar_init(bars + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+
+  // ---- this warp's stages: keys c0 + 32 (warp + 4 i)
+  const int n_stages = c1 > c0 + warp * kKeys ? (c1 - c0 - warp * kKeys + kKeys * kWarps - 1) /
+                                                    (kKeys * kWarps)
+                                              : 0;
+  const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
+  const int page_rows = 1 << p.page_shift;
+  const int piece = min(page_rows, kKeys);   // keys of one copy
+  const int pieces = kKeys / piece;          // 1 or 2
+  const int64_t side_code = (int64_t)a.cache.kv_heads * page_rows * S::kCodeRow;
+  const int64_t side_scale = (int64_t)a.cache.kv_heads * page_rows * S::kScaleRow;
+  // lane l < 4 * pieces copies part l & 3 (K codes, K scales, V codes, V scales) of piece l >> 2
+  const int part = lane & 3, my_piece = lane >> 2;
+  auto page_of = [&](int i) -> int {  // the page of this lane's piece of stage i, or -1
+    const int k = c0 + (warp + i * kWarps) * kKeys + my_piece * piece;
+    if (my_piece >= pieces || i >= n_stages || k >= tile.end) return -1;
+    const int pg = __ldg(table + (k >> p.page_shift));
+    return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
+  };
+  auto issue = [&](int i, int pg) {
+    const uint32_t bar = bars + 8 * (i % S::kStages);
+    const uint32_t live = __ballot_sync(0xFFFFFFFFu, pg >= 0 && my_piece < pieces);
+    if (lane == 0)
+      mbar_expect_tx(bar, (uint32_t)(__popc(live) / 4) * (uint32_t)(S::kStage / kKeys * piece));
+    __syncwarp();
+    if (pg >= 0 && my_piece < pieces) {
+      const int k = c0 + (warp + i * kWarps) * kKeys + my_piece * piece;
+      const int64_t row = (int64_t)head * page_rows + (k & (page_rows - 1));
+      const bool scales = part & 1, value = part & 2;
+      const uint32_t bytes = piece * (scales ? S::kScaleRow : S::kCodeRow);
+      const uint8_t* src =
+          scales ? a.cache.scales + pg * a.cache.scales_page_stride + (value ? side_scale : 0) +
+                       row * S::kScaleRow
+                 : a.cache.codes + pg * a.cache.codes_page_stride + (value ? side_code : 0) +
+                       row * S::kCodeRow;
+      const uint32_t dst = ring + (i % S::kStages) * S::kStage +
+                           (value ? S::kKCodes + S::kKScales : 0) + (scales ? S::kKCodes : 0) +
+                           my_piece * bytes;
+      bulk_load(dst, src, bytes, bar);
+    }
+    return live;
+  };
+  // Which pieces of a stage in flight came, two bits a stage (bit 0: piece 0).
+  uint32_t present = 0;
+  auto note = [&](int i, uint32_t live) {
+    const int at = 2 * (i % S::kStages);
+    present = (present & ~(3u << at)) | (((live & 1u) | ((live >> 3) & 2u)) << at);
+  };
+  for (int i = 0; i < S::kStages && i < n_stages; ++i) note(i, issue(i, page_of(i)));
+  int next_page = page_of(S::kStages);
+
+  // ---- queries: B fragments of f16, permuted as the keys are
+  uint32_t q[kNT][S::kKSteps][2];
+  float scale[kNT][2];
+  int lo_key[kNT][2], hi_key[kNT][2];
+  float acc[kNT][kD / 16][4], m[kNT][2], l[kNT][2];
+  const float to_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+#pragma unroll
+  for (int n = 0; n < kNT; ++n) {
+    const int r = n * 8 + g;
+    uint32_t w[kQuarter / 2];
+    const bool live = r < tile.rows;
+    if (live) {
+      const int row = tile.row0 + r, token = row / p.group, hh = row - token * p.group;
+      const uint16_t* src = a.q.p + (int64_t)(tile.first_token + token) * a.q.token_stride +
+                            (int64_t)(head * p.group + hh) * a.q.head_stride + t * kQuarter;
+#pragma unroll
+      for (int j = 0; j < kQuarter / 8; ++j)
+        *reinterpret_cast<uint4*>(&w[4 * j]) = *(reinterpret_cast<const uint4*>(src) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuarter / 2; ++j) w[j] = 0;
+    }
+    float row_scale = to_log2;
+    if (a.dtype == kDTypeBF16) {
+      // bf16 has a wider range than f16: scale the row by a power of two that
+      // brings its largest element into [1, 2); elements above 2^-17 of it
+      // stay exact, the others are off by less than 2^-25 of it.
+      uint32_t big = 0;
+#pragma unroll
+      for (int j = 0; j < kQuarter / 2; ++j)
+        big = max(big, max((w[j] << 16) & 0x7FFFFFFFu, w[j] & 0x7FFF0000u));
+      big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      const int e = (int)(big >> 23);
+      // exponents 1..253: 2^(127 - e) is a normal number; zero, subnormal, the
+      // largest and non-finite rows are left as they are
+      const bool sized = e >= 1 && e <= 253;
+      const float down = sized ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+      row_scale = sized ? to_log2 * __uint_as_float((uint32_t)e << 23) : to_log2;
+#pragma unroll
+      for (int j = 0; j < kQuarter / 2; ++j)
+        w[j] = pack_h2(__uint_as_float(w[j] << 16) * down,
+                       __uint_as_float(w[j] & 0xFFFF0000u) * down);
+    }
+#pragma unroll
+    for (int j = 0; j < S::kKSteps; ++j) {
+      q[n][j][0] = w[2 * j];
+      q[n][j][1] = w[2 * j + 1];
+    }
+    // columns 2t, 2t + 1 of the score tile are rows n * 8 + 2t, + 1
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      scale[n][c] = __shfl_sync(0xFFFFFFFFu, row_scale, (2 * t + c) * 4);
+      const int rr = n * 8 + 2 * t + c;
+      const int pos = tile.offset + (tile.row0 + rr) / p.group;
+      const bool there = rr < tile.rows;
+      hi_key[n][c] = !there ? -1 : a.causal ? min(pos, tile.end - 1) : tile.end - 1;
+      lo_key[n][c] = a.window >= 0 ? pos - a.window : 0;
+      m[n][c] = -INFINITY;
+      l[n][c] = 0.0f;
+    }
+#pragma unroll
+    for (int d = 0; d < kD / 16; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[n][d][c] = 0.0f;
+  }
+
+  // ---- one pass over this warp's stages
+  // Row rho of a 16-key group's tile is key pi(rho): pi(2u) = u, pi(2u + 1) =
+  // u + 4, pi(8 + 2u) = u + 8, pi(9 + 2u) = u + 12, so that the values a
+  // thread pairs lie in rows t, t + 4, t + 8, t + 12.
+  const int key_a = (g >> 1) + (g & 1) * 4;  // pi(g); pi(g + 8) = pi(g) + 8
+  bool ok = true;
+  for (int i = 0; i < n_stages; ++i) {
+    const int slot = i % S::kStages;
+    const int k0 = c0 + (warp + i * kWarps) * kKeys;
+    const int page_ahead = next_page;
+    next_page = page_of(i + 1 + S::kStages);
+    if (!mbar_wait(bars + 8 * slot, (i / S::kStages) & 1)) {
+      // give up: the copies still in flight get their (bounded) time to land
+      for (int j = i; j < n_stages && j < i + S::kStages; ++j)
+        mbar_wait(bars + 8 * (j % S::kStages), (j / S::kStages) & 1);
+      ok = false;
+      break;
+    }
+    const uint8_t* st = smem + warp * S::kRing + slot * S::kStage;
+    const uint8_t* kc = st;
+    const uint8_t* ks = st + S::kKCodes;
+    const uint8_t* vc = st + S::kKCodes + S::kKScales;
+    const uint8_t* vs = vc + S::kKCodes;
+    const uint32_t came = (present >> (2 * slot)) & 3u;
+    const bool masked = k0 < tile.all_beg || k0 + kKeys > tile.all_end || k0 + kKeys > c1 ||
+                        came != (pieces == 2 ? 3u : 1u);
+
+    // S^T = K Q^T
+    float s[2][kNT][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t kw[2][kKWords], sc[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int row = h * 16 + key_a + 8 * r;
+        const uint8_t* src = kc + row * S::kCodeRow + t * (kQuarter / 2);
+        if constexpr (kKWords == 2) {
+          *reinterpret_cast<uint2*>(kw[r]) = *reinterpret_cast<const uint2*>(src);
+          sc[r] = ks[row * S::kScaleRow + t];
+        } else {
+#pragma unroll
+          for (int j = 0; j < kKWords / 4; ++j)
+            *reinterpret_cast<uint4*>(&kw[r][4 * j]) = *(reinterpret_cast<const uint4*>(src) + j);
+          if constexpr (kKWords == 4)
+            sc[r] = *reinterpret_cast<const uint16_t*>(ks + row * S::kScaleRow + 2 * t);
+          else
+            sc[r] = *reinterpret_cast<const uint32_t*>(ks + row * S::kScaleRow + 4 * t);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[h][n][c] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < S::kKSteps; ++j) {
+        uint32_t f[2];  // the scale of this step's block, twice
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t two = e4m3_h2(sc[r] >> (16 * (j / 8)));
+          f[r] = __byte_perm(two, two, (j / 4) & 1 ? 0x3232 : 0x1010);
+        }
+        const int word = j / 2, byte = 2 * (j & 1);
+        const uint32_t a0 = mul_h2(e2m1_h2(kw[0][word], byte), f[0]);
+        const uint32_t a1 = mul_h2(e2m1_h2(kw[1][word], byte), f[1]);
+        const uint32_t a2 = mul_h2(e2m1_h2(kw[0][word], byte + 1), f[0]);
+        const uint32_t a3 = mul_h2(e2m1_h2(kw[1][word], byte + 1), f[1]);
+#pragma unroll
+        for (int n = 0; n < kNT; ++n) mma16816(s[h][n], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
+      }
+    }
+
+    // softmax over this stage's keys, in units of log2
+    uint32_t pt[2][kNT][2];  // P^T as B fragments
+    bool grow = false;
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v = s[h][n][c] * scale[n][c & 1];
+          if (masked) {
+            const int key = k0 + h * 16 + key_a + 8 * (c >> 1);
+            const bool here = (came >> (pieces == 2 ? h : 0)) & 1u;
+            if (!here || key >= c1 || key > hi_key[n][c & 1] || key < lo_key[n][c & 1])
+              v = -INFINITY;
+          }
+          s[h][n][c] = v;
+          mx[c & 1] = fmaxf(mx[c & 1], v);
+        }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 4));
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 8));
+        mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 16));
+        grow |= mx[c] > m[n][c] + kSlack;
+      }
+      if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float mn = fmaxf(m[n][c], mx[c]);
+          const float f = mn == -INFINITY ? 1.0f : ex2(m[n][c] - mn);
+          m[n][c] = mn;
+          l[n][c] *= f;
+#pragma unroll
+          for (int d = 0; d < kD / 16; ++d) {
+            acc[n][d][c] *= f;
+            acc[n][d][c + 2] *= f;
+          }
+        }
+      }
+      const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - kShift;
+      const float m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - kShift;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float p0 = ex2(s[h][n][0] - m0), p1 = ex2(s[h][n][1] - m1);
+        const float p2 = ex2(s[h][n][2] - m0), p3 = ex2(s[h][n][3] - m1);
+        l[n][0] += p0 + p2;
+        l[n][1] += p1 + p3;
+        pt[h][n][0] = transpose8(pack_h2(p0, p1));
+        pt[h][n][1] = transpose8(pack_h2(p2, p3));
+      }
+    }
+
+    // O^T += V^T P^T
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t vw[4][kVWords], sc[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = h * 16 + t + 4 * r;
+        const uint8_t* src = vc + row * S::kCodeRow + g * (kD / 16);
+        if constexpr (kD == 64) {
+          vw[r][0] = *reinterpret_cast<const uint32_t*>(src);
+          sc[r] = vs[row * S::kScaleRow + (g >> 1)];
+        } else if constexpr (kD == 128) {
+          *reinterpret_cast<uint2*>(vw[r]) = *reinterpret_cast<const uint2*>(src);
+          sc[r] = vs[row * S::kScaleRow + g];
+        } else {
+          *reinterpret_cast<uint4*>(vw[r]) = *reinterpret_cast<const uint4*>(src);
+          sc[r] = *reinterpret_cast<const uint16_t*>(vs + row * S::kScaleRow + 2 * g);
+        }
+        // what lies behind the last key may hold anything, NaN scales too
+        if (masked) {
+          const int key = k0 + row;
+          const bool here = (came >> (pieces == 2 ? h : 0)) & 1u;
+          if (!here || key >= c1 || key < tile.beg) sc[r] = 0;
+        }
+      }
+      // scales of key pairs (t, t + 4) and (t + 8, t + 12)
+      uint32_t f[2][kD == 256 ? 2 : 1];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f[u][0] = e4m3_h2((sc[2 * u] & 0xFF) | ((sc[2 * u + 1] & 0xFF) << 8));
+        if constexpr (kD == 256) f[u][1] = e4m3_h2((sc[2 * u] >> 8) | (sc[2 * u + 1] & 0xFF00));
+      }
+#pragma unroll
+      for (int w = 0; w < kVWords; ++w) {
+        uint32_t even[2], odd[2];  // bytes (code of the first key, code of the second) of even / odd d
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t x = vw[2 * u][w], y = vw[2 * u + 1][w];
+          even[u] = (x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u);
+          odd[u] = ((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u);
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          // tile w * 4 + b: row g is d = g * D/8 + 8 w + 2 b, row g + 8 the next
+          const int fi = kD == 256 ? w / 2 : 0;
+          const uint32_t a0 = mul_h2(e2m1_h2(even[0], b), f[0][fi]);
+          const uint32_t a1 = mul_h2(e2m1_h2(odd[0], b), f[0][fi]);
+          const uint32_t a2 = mul_h2(e2m1_h2(even[1], b), f[1][fi]);
+          const uint32_t a3 = mul_h2(e2m1_h2(odd[1], b), f[1][fi]);
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+            mma16816(acc[n][w * 4 + b], a0, a1, a2, a3, pt[h][n][0], pt[h][n][1]);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage before it is filled again
+    if (i + S::kStages < n_stages) note(i + S::kStages, issue(i + S::kStages, page_ahead));
+  }
+  if (!ok && lane == 0 && a.status) atomicCAS(a.status, 0, 1);
+
+  // ---- merge the warps through shared memory
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      l[n][c] += __shfl_xor_sync(0xFFFFFFFFu, l[n][c], 4);
+      l[n][c] += __shfl_xor_sync(0xFFFFFFFFu, l[n][c], 8);
+      l[n][c] += __shfl_xor_sync(0xFFFFFFFFu, l[n][c], 16);
+    }
+  __syncthreads();  // the rings are free
+  float* mine = reinterpret_cast<float*>(smem) + warp * kRows * (kD + 2);
+#pragma unroll
+  for (int n = 0; n < kNT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float* row = mine + (n * 8 + 2 * t + c) * (kD + 2);
+      if (g == 0) {
+        row[kD] = m[n][c];
+        row[kD + 1] = l[n][c];
+      }
+#pragma unroll
+      for (int d = 0; d < kD / 16; ++d) {
+        row[g * (kD / 8) + 2 * d] = acc[n][d][c];
+        row[g * (kD / 8) + 2 * d + 1] = acc[n][d][c + 2];
+      }
+    }
+  __syncthreads();
+  const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
+  const float* all = reinterpret_cast<const float*>(smem);
+  constexpr int kStride = kRows * (kD + 2);
+  for (int at = threadIdx.x; at < tile.rows * (kD / 2); at += kThreads) {
+    const int r = at / (kD / 2), d = (at % (kD / 2)) * 2;
+    const float* x = all + r * (kD + 2);
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, x[w * kStride + kD]);
+    float o[2] = {0.0f, 0.0f}, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = mm == -INFINITY ? 0.0f : ex2(x[w * kStride + kD] - mm);
+      sum += f * x[w * kStride + kD + 1];
+      o[0] += f * x[w * kStride + d];
+      o[1] += f * x[w * kStride + d + 1];
+    }
+    const int row = tile.row0 + r, token = tile.first_token + row / p.group;
+    const int qh = head * p.group + row % p.group;
+    const int64_t out_row = (int64_t)token * a.q_heads + qh;
+    if (p.splits == 1) {
+      // a row that sees no key is zero
+      const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;
+      o[0] *= inv;
+      o[1] *= inv;
+      store16(a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride + d,
+              o, a.dtype);
+      if (d == 0 && a.lse)
+        a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+    } else {
+      const int64_t at_row = (int64_t)split * a.tokens * a.q_heads + out_row;
+      *reinterpret_cast<float2*>(p.part_o + at_row * kD + d) = make_float2(o[0], o[1]);
+      if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at_row * 2) = make_float2(mm, sum);
+    }
+  }
+}
+
+// Joins the splits of a tile's rows in their order: one warp per row.
+template <int kD>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile_rows) {
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.z, seq = blockIdx.x / p.tiles;
+  Tile tile;
+  if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile)) return;
+  const int splits = used_splits(p, tile);
+  const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
+  for (int r = blockIdx.y * kWarps + warp; r < tile.rows; r += gridDim.y * kWarps) {
+    const int row = tile.row0 + r, token = tile.first_token + row / p.group;
+    const int qh = head * p.group + row % p.group;
+    const int64_t out_row = (int64_t)token * a.q_heads + qh;
+    const int64_t step = a.tokens * a.q_heads;
+    float mm = -INFINITY;
+    for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, p.part_ml[(s * step + out_row) * 2]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
+    float sum = 0.0f, acc[kD / 32];
+#pragma unroll
+    for (int j = 0; j < kD / 32; ++j) acc[j] = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * step + out_row) * 2);
+      const float f = mm == -INFINITY ? 0.0f : ex2(ml.x - mm);
+      sum += f * ml.y;
+      const float* o = p.part_o + (s * step + out_row) * kD;
+#pragma unroll
+      for (int j = 0; j < kD / 64; ++j) {
+        const float2 v = *reinterpret_cast<const float2*>(o + j * 64 + lane * 2);
+        acc[2 * j] += f * v.x;
+        acc[2 * j + 1] += f * v.y;
+      }
+    }
+    const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;
+    uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
+#pragma unroll
+    for (int j = 0; j < kD / 64; ++j) {
+      const float v[2] = {acc[2 * j] * inv, acc[2 * j + 1] * inv};
+      store16(dst + j * 64 + lane * 2, v, a.dtype);
+    }
+    if (lane == 0 && a.lse)
+      a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+  }
+}
+
+int log2i(int v) {
+  int s = 0;
+  while ((1 << s) < v) ++s;
+  return s;
+}
+
+struct Plan {
+  int rows;  // of a tile
+  int tiles, splits, chunk;
+};
+
+Plan plan_of(const AttendArgs& a, int device_sms) {
+  Plan pl;
+  const int group = a.q_heads / a.cache.kv_heads;
+  const int64_t rows = (int64_t)a.max_query_len * group;
+  pl.rows = rows <= 8 ? 8 : rows <= 16 || a.cache.head_size == 256 ? 16 : 32;
+  pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
+  int64_t span = a.max_seq_len;
+  if (a.window >= 0 && span > (int64_t)a.window + a.max_query_len + kKeys)
+    span = (int64_t)a.window + a.max_query_len + kKeys;
+  const int64_t units = (int64_t)a.seqs * pl.tiles * a.cache.kv_heads;
+  const int64_t want = (int64_t)device_sms * 3 * 4;
+  int64_t splits = (want + units - 1) / units;
+  constexpr int kStep = kKeys * kWarps;
+  int64_t chunk = ((span + splits - 1) / splits + kStep - 1) / kStep * kStep;
+  if (chunk < 2 * kStep) chunk = 2 * kStep;
+  pl.chunk = (int)chunk;
+  // the first key of a windowed tile is rounded down to a stage
+  pl.splits = (int)((span + kKeys - 1 + chunk - 1) / chunk);
+  if (pl.splits < 1) pl.splits = 1;
+  return pl;
+}
+
+int64_t part_rows(const AttendArgs& a, const Plan& pl) {
+  return pl.splits > 1 ? (int64_t)pl.splits * a.tokens * a.q_heads : 0;
+}
+
+template <int kD, int kNT>
+cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
+  constexpr int kSmem = smem_bytes<kD, kNT>();
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(decode_kernel<kD, kNT>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
+  decode_kernel<kD, kNT><<<grid, kThreads, kSmem, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  const dim3 jgrid(grid.x, kNT * 8 / kWarps, grid.z);
+  join_kernel<kD><<<jgrid, kThreads, 0, stream>>>(p, kNT * 8);
+  return cudaGetLastError();
+}
+
+template <int kD>
+cudaError_t launch_rows(const Params& p, int rows, cudaStream_t stream) {
+  if (rows == 8) return launch_decode<kD, 1>(p, stream);
+  if (rows == 16) return launch_decode<kD, 2>(p, stream);
+  if constexpr (kD < 256) return launch_decode<kD, 4>(p, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+int64_t attend_workspace_bytes(const AttendArgs& a, int device_sms) {
+  const Plan pl = plan_of(a, device_sms);
+  return part_rows(a, pl) * (a.cache.head_size + 2) * (int64_t)sizeof(float);
+}
+
+cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stream) {
+  const Plan pl = plan_of(a, device_sms);
+  Params p;
+  p.a = a;
+  p.group = a.q_heads / a.cache.kv_heads;
+  p.tiles = pl.tiles;
+  p.splits = pl.splits;
+  p.chunk = pl.chunk;
+  p.page_shift = log2i(a.cache.page_size);
+  p.part_o = a.workspace;
+  p.part_ml = a.workspace ? a.workspace + part_rows(a, pl) * a.cache.head_size : nullptr;
+  if (a.cache.head_size == 64) return launch_rows<64>(p, pl.rows, stream);
+  if (a.cache.head_size == 128) return launch_rows<128>(p, pl.rows, stream);
+  return launch_rows<256>(p, pl.rows, stream);
+}
+
+}  // namespace kv
+}  // namespace ssw

@@ -1,0 +1,239 @@
+"""NVFP4 KV cache: rotary positions and the scale-sweep quantizer in one write.
+
+Between the qkv projection and attention, a decoder layer rotates its query
+and key heads and stores keys and values.  This module does both in one
+launch, holding the cache in the format of the framework's activations: E2M1
+codes with one E4M3 scale per 16 elements, the scale chosen by the
+``scalesweep_mse`` sweep.  The stored bytes are those of
+``scalesweep_mse_nvfp4_quant`` on the rotated 16-bit keys and the values.
+
+Layout (``alloc_kv_cache``): pages of ``page_size`` tokens,
+
+* ``codes``  uint8 ``[num_pages, 2, kv_heads, page_size, head_size / 2]``,
+* ``scales`` float8_e4m3fn ``[num_pages, 2, kv_heads, page_size, head_size / 16]``,
+
+index 0 of the second axis holding keys and index 1 values.  The first axis
+may be strided: ``codes[layer]`` of a cache allocated for all layers is a
+layer's cache.  ``kv_input_scale`` is a float32 ``[2]`` tensor with the
+multipliers (``256 * 6 / amax``) of the layer's keys and values; a stored value
+stands for ``code * scale / multiplier``.  A token's slot is
+``page * page_size + row``.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+PAGE_SIZES = (16, 32, 64, 128)
+HEAD_SIZES = (64, 128, 256)
+
+
+def alloc_kv_cache(num_pages: int, page_size: int, kv_heads: int, head_size: int,
+                   device: torch.device | str = "cuda", num_layers: int | None = None):
+    """(codes, scales) of an empty cache; with ``num_layers`` a leading layer
+    axis.  Uninitialised, like the pages of any cache."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if head_size not in HEAD_SIZES:
+        raise ValueError(f"head_size must be one of {HEAD_SIZES}, got {head_size}")
+    if num_pages < 1 or kv_heads < 1 or (num_layers is not None and num_layers < 1):
+        raise ValueError("num_pages, kv_heads and num_layers must be positive")
+    shape = ((num_layers,) if num_layers is not None else ()) + (num_pages, 2, kv_heads, page_size)
+    return (torch.empty(shape + (head_size // 2,), dtype=torch.uint8, device=device),
+            torch.empty(shape + (head_size // 16,), dtype=torch.float8_e4m3fn, device=device))
+
+
+def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000.0,
+                         scaling: dict | None = None,
+                         device: torch.device | str = "cuda") -> torch.Tensor:
+    """float32 ``[max_position, rotary_dim]``: the cosines, then the sines, of
+    ``position * frequency``, formed in binary64 (a binary32 angle is off by
+    4e-3 at position 100000).
+
+    ``scaling`` follows the ``rope_scaling`` of a model's configuration, by its
+    ``rope_type``: ``linear`` (``factor``), ``llama3`` (``factor``,
+    ``low_freq_factor``, ``high_freq_factor``,
+    ``original_max_position_embeddings``) or ``yarn`` (``factor``,
+    ``original_max_position_embeddings``, optionally ``beta_fast``,
+    ``beta_slow`` and ``attention_factor``, which multiplies both tables).
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if max_position < 1:
+        raise ValueError(f"max_position must be positive, got {max_position}")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    freq = float(base) ** (-i / rotary_dim)
+    mult = 1.0
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "linear":
+        freq = freq / float(scaling["factor"])
+    elif kind == "llama3":
+        factor, original = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        wave = 2 * math.pi / freq
+        smooth = (original / wave - low) / (high - low)
+        between = (1 - smooth) * freq / factor + smooth * freq
+        freq = torch.where(wave > original / low, freq / factor,
+                           torch.where(wave < original / high, freq, between))
+    elif kind == "yarn":
+        factor, original = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
+
+        def dim_of(turns):  # the pair that turns this often over the original length
+            return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low = max(math.floor(dim_of(float(scaling.get("beta_fast", 32.0)))), 0)
+        high = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1.0)))), rotary_dim - 1)
+        ramp = ((i / 2 - low) / max(high - low, 0.001)).clamp(0, 1)
+        freq = freq / factor * ramp + freq * (1 - ramp)
+        mult = scaling.get("attention_factor")
+        mult = 0.1 * math.log(factor) + 1.0 if mult is None else float(mult)
+    elif kind != "default":
+        raise ValueError(f"unsupported rope_type {kind!r}")
+    angle = torch.arange(max_position, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos() * mult, angle.sin() * mult], dim=-1).float()
+
+
+def cache_struct(codes: torch.Tensor, scales: torch.Tensor,
+                 kv_input_scale: torch.Tensor | None) -> _lib.KVCache:
+    """Check one layer's cache tensors and describe them to the C ABI."""
+    if codes.dim() != 5 or scales.dim() != 5:
+        raise ValueError("codes and scales must be [num_pages, 2, kv_heads, page_size, ..] tensors")
+    pages, two, heads, page, half = codes.shape
+    if codes.dtype != torch.uint8 or scales.dtype != torch.float8_e4m3fn:
+        raise ValueError("codes must be uint8 and scales float8_e4m3fn, got "
+                         f"{codes.dtype} and {scales.dtype}")
+    if two != 2 or scales.shape != (pages, 2, heads, page, half // 8):
+        raise ValueError("codes must be [num_pages, 2, kv_heads, page_size, head_size/2] and scales "
+                         f"[.., head_size/16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+    dev = codes.device
+    if dev.type != "cuda":
+        raise ValueError("codes must be a CUDA tensor (there is no CPU implementation)")
+    if scales.device != dev:
+        raise ValueError(f"scales must be on {dev}, got {scales.device}")
+    sc, ss = codes.stride(), scales.stride()
+    row, srow = page * half, page * (half // 8)
+    if (sc[1:] != (heads * row, row, half, 1)
+            or ss[1:] != (heads * srow, srow, half // 8, 1)):
+        raise ValueError("codes and scales must be contiguous within a page")
+    mult = 0
+    if kv_input_scale is not None:
+        if (kv_input_scale.dtype != torch.float32 or kv_input_scale.shape != (2,)
+                or kv_input_scale.device != dev or kv_input_scale.stride(0) != 1):
+            raise ValueError(f"kv_input_scale must be a contiguous float32 tensor of shape [2] on {dev}")
+        mult = kv_input_scale.data_ptr()
+    return _lib.KVCache(codes.data_ptr(), scales.data_ptr(), sc[0], ss[0], mult, pages, page, heads,
+                        half * 2)
+
+
+def heads_struct(name: str, t: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
+                 device: torch.device) -> _lib.KVHeads:
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}, got {t.dtype} "
+                         f"{list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    st, sh, sd = t.stride()
+    # the stride of an axis of length 1 says nothing, and may be anything
+    if shape[0] <= 1:
+        st = 0
+    if shape[1] <= 1:
+        sh = 0
+    if sd != 1 or st % 8 or sh % 8:
+        raise ValueError(f"{name}: the last dimension must be contiguous, the other strides "
+                         "multiples of 8")
+    return _lib.KVHeads(t.data_ptr(), st, sh)
+
+
+def check_distinct(name: str, t: torch.Tensor) -> None:
+    """Refuse an output whose elements share memory (an expanded tensor)."""
+    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} must not be an expanded tensor")
+
+
+def _check_index(name: str, t: torch.Tensor, n: int, device: torch.device) -> None:
+    if t.dtype != torch.int64 or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int64 tensor of shape [{n}] on {device}")
+
+
+def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
+                                         value: torch.Tensor, positions: torch.Tensor,
+                                         cos_sin_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                                         kv_input_scale: torch.Tensor, codes: torch.Tensor,
+                                         scales: torch.Tensor, *, is_neox: bool = True,
+                                         query_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate ``query`` [T, Hq, D] and ``key`` [T, Hkv, D], and quantize the
+    rotated keys and ``value`` into the cache's rows ``slot_mapping`` [T].
+
+    The three are bf16 or f16, and may be slices of a qkv projection's output
+    (last dimension contiguous, other strides multiples of 8).  ``positions``
+    and ``slot_mapping`` are int64 [T].  ``cos_sin_cache`` is float32
+    ``[max_position, rotary_dim]`` (:func:`rotary_cos_sin_cache`), ``rotary_dim``
+    a multiple of 16 up to D; elements past it are not rotated.  ``is_neox``
+    pairs element i with i + rotary_dim / 2, otherwise 2i with 2i + 1.
+
+    Returns the rotated query: ``query_out`` if given (``query`` itself rotates
+    in place), else a new contiguous tensor.  ``key`` and ``value`` are only
+    read.  Rows whose slot is negative or past the last page are padding: not
+    stored.  Slots must be distinct.  A position outside the table gives NaN in
+    the query, and that token is not stored."""
+    cache = cache_struct(codes, scales, kv_input_scale)
+    if kv_input_scale is None:
+        raise ValueError("kv_input_scale is required")
+    dev = codes.device
+    if query.dim() != 3:
+        raise ValueError(f"query must be [T, heads, head_size], got shape {tuple(query.shape)}")
+    tokens, hq, d = query.shape
+    if d != cache.head_size:
+        raise ValueError(f"query has head size {d}, the cache {cache.head_size}")
+    dtype = _lib.dtype_code(query)
+    kv_shape = (tokens, cache.kv_heads, d)
+    q = heads_struct("query", query, (tokens, hq, d), query.dtype, dev)
+    k = heads_struct("key", key, kv_shape, query.dtype, dev)
+    v = heads_struct("value", value, kv_shape, query.dtype, dev)
+    _check_index("positions", positions, tokens, dev)
+    _check_index("slot_mapping", slot_mapping, tokens, dev)
+    if (cos_sin_cache.dtype != torch.float32 or cos_sin_cache.dim() != 2
+            or cos_sin_cache.device != dev or not cos_sin_cache.is_contiguous()):
+        raise ValueError("cos_sin_cache must be a contiguous float32 tensor [max_position, "
+                         f"rotary_dim] on {dev}")
+    if query_out is None:
+        query_out = torch.empty((tokens, hq, d), dtype=query.dtype, device=dev)
+    o = heads_struct("query_out", query_out, (tokens, hq, d), query.dtype, dev)
+    check_distinct("query_out", query_out)
+    max_position, rotary_dim = cos_sin_cache.shape
+    with _lib.on_device(dev):
+        st = _lib.lib().ssw_rotary_scalesweep_mse_nvfp4_kv_write(
+            ctypes.byref(cache), dtype, tokens, hq, ctypes.byref(q), ctypes.byref(k),
+            ctypes.byref(v), ctypes.byref(o), positions.data_ptr(), cos_sin_cache.data_ptr(),
+            max_position, rotary_dim, bool(is_neox), slot_mapping.data_ptr(),
+            _lib.stream_handle(dev))
+    _lib.check(st)
+    return query_out
+
+
+def nvfp4_kv_gather(codes: torch.Tensor, scales: torch.Tensor, kv_input_scale: torch.Tensor,
+                    slot_mapping: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """The keys and values stored at ``slot_mapping`` [T], as 16-bit floats:
+    (key, value), each [T, kv_heads, head_size] and contiguous.  Zeros for a
+    slot outside the cache.  For a cache's readers that want plain keys and
+    values: another engine's cache, or a check of what the quantizer kept."""
+    cache = cache_struct(codes, scales, kv_input_scale)
+    if kv_input_scale is None:
+        raise ValueError("kv_input_scale is required")
+    dev = codes.device
+    if dtype not in _lib.DTYPE_CODES:
+        raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
+    _check_index("slot_mapping", slot_mapping, slot_mapping.numel(), dev)
+    n = slot_mapping.numel()
+    shape = (n, cache.kv_heads, cache.head_size)
+    key = torch.empty(shape, dtype=dtype, device=dev)
+    value = torch.empty(shape, dtype=dtype, device=dev)
+    with _lib.on_device(dev):
+        st = _lib.lib().ssw_nvfp4_kv_gather(ctypes.byref(cache), _lib.DTYPE_CODES[dtype], n,
+                                            slot_mapping.data_ptr(), key.data_ptr(),
+                                            value.data_ptr(), _lib.stream_handle(dev))
+    _lib.check(st)
+    return key, value
