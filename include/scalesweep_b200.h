@@ -404,6 +404,68 @@ int ssw_nvfp4_paged_attention(const ssw_kv_cache* cache, const ssw_kv_attention*
                               const ssw_kv_heads* query, const ssw_kv_heads* out, void* workspace,
                               int64_t workspace_bytes, void* stream);
 
+/*
+ * Page tables of a cache, all on the device: reference counts of its pages,
+ * each sequence's pages in order (-1: none) and its number of tokens.  An empty
+ * sequence has length 0 and a row of -1.  A page is free while nothing refers
+ * to it; pages are taken lowest first, in the order of the requests.  A call
+ * that cannot be served as a whole changes nothing, and status (may be null)
+ * becomes, unless it is nonzero already: 1 not enough free pages, 2 a sequence
+ * out of range, named twice, or (fork) a child that is not empty, 3 a sequence
+ * longer than its row.  A pool is the cache's bytes over all layers.
+ */
+typedef struct {
+  int32_t* refcount;    /* [num_pages] */
+  int32_t* block_table; /* [max_seqs, columns] */
+  int64_t table_stride; /* elements between sequences */
+  int32_t* seq_lens;    /* [max_seqs] */
+  int32_t* status;
+  int32_t num_pages;
+  int32_t max_seqs;
+  int32_t columns;
+  int32_t page_size;
+} ssw_kv_pages;
+
+typedef struct {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t codes_layer_stride; /* bytes; multiples of 16, as all strides and sizes here */
+  int64_t scales_layer_stride;
+  int64_t codes_page_stride;
+  int64_t scales_page_stride;
+  int64_t codes_page_bytes;
+  int64_t scales_page_bytes;
+  int64_t num_pages;
+  int32_t layers;
+} ssw_kv_pool;
+
+/* Workspace that serves any of the calls below: n requests for total_tokens
+ * new tokens in a pool of num_pages.  Calls that may overlap need their own. */
+int64_t ssw_kv_pages_workspace_bytes(int64_t n, int64_t total_tokens, int page_size,
+                                     int64_t num_pages);
+/* Child i becomes a copy of parent i: the parent's full pages are shared, a
+ * part-filled last page is copied.  A parent may be named more than once. */
+int ssw_kv_pages_fork(const ssw_kv_pages* tables, const ssw_kv_pool* pool, int64_t n,
+                      const int32_t* parents, const int32_t* children, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+/* The sequences become empty; pages that nothing refers to any more are free.
+ * A sequence named twice is freed once; one out of range is passed over. */
+int ssw_kv_pages_free(const ssw_kv_pages* tables, int64_t n, const int32_t* seqs, void* stream);
+/* new_tokens[i] tokens more for sequence seqs[i]; slot_mapping [total_tokens]
+ * gets their slots, sequence by sequence (-1 where the call was not served).
+ * total_tokens is the sum of new_tokens. */
+int ssw_kv_pages_extend(const ssw_kv_pages* tables, int64_t n, const int32_t* seqs,
+                        const int32_t* new_tokens, int64_t total_tokens, int64_t* slot_mapping,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+/* With L pages in use, those numbered L and above move, in order, into the
+ * free ones below: afterwards pages 0 .. L - 1 are in use. */
+int ssw_kv_pages_compact(const ssw_kv_pages* tables, const ssw_kv_pool* pool, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+/* Page source[i] is copied to target[i] in every layer.  Targets must be
+ * distinct and no source may be a target; pairs out of range are passed over. */
+int ssw_kv_pages_copy(const ssw_kv_pool* pool, int64_t n, const int32_t* source,
+                      const int32_t* target, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

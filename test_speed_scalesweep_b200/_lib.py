@@ -52,6 +52,12 @@ _SIGNATURES = {
     "ssw_rotary_scalesweep_mse_nvfp4_kv_write": (_int, [_c_p, _int, _i64, _int, _c_p, _c_p, _c_p, _c_p,
                                                         _c_p, _c_p, _i64, _int, _int, _c_p, _c_p]),
     "ssw_nvfp4_kv_gather": (_int, [_c_p, _int, _i64, _c_p, _c_p, _c_p, _c_p]),
+    "ssw_kv_pages_workspace_bytes": (_i64, [_i64, _i64, _int, _i64]),
+    "ssw_kv_pages_fork": (_int, [_c_p, _c_p, _i64, _c_p, _c_p, _c_p, _i64, _c_p]),
+    "ssw_kv_pages_free": (_int, [_c_p, _i64, _c_p, _c_p]),
+    "ssw_kv_pages_extend": (_int, [_c_p, _i64, _c_p, _c_p, _i64, _c_p, _c_p, _i64, _c_p]),
+    "ssw_kv_pages_compact": (_int, [_c_p, _c_p, _c_p, _i64, _c_p]),
+    "ssw_kv_pages_copy": (_int, [_c_p, _i64, _c_p, _c_p, _c_p]),
     "ssw_nvfp4_paged_attention_workspace_bytes": (_i64, [_c_p, _c_p, _int]),
     "ssw_nvfp4_paged_attention": (_int, [_c_p, _c_p, _int, _c_p, _c_p, _c_p, _i64, _c_p]),
 }
@@ -78,6 +84,22 @@ class KVAttention(ctypes.Structure):
                 ("q_heads", ctypes.c_int32), ("max_query_len", ctypes.c_int32),
                 ("max_seq_len", ctypes.c_int32), ("causal", ctypes.c_int32),
                 ("window", ctypes.c_int32), ("softmax_scale", _f32)]
+
+
+class KVPages(ctypes.Structure):
+    """``ssw_kv_pages``."""
+    _fields_ = [("refcount", _c_p), ("block_table", _c_p), ("table_stride", _i64),
+                ("seq_lens", _c_p), ("status", _c_p), ("num_pages", ctypes.c_int32),
+                ("max_seqs", ctypes.c_int32), ("columns", ctypes.c_int32),
+                ("page_size", ctypes.c_int32)]
+
+
+class KVPool(ctypes.Structure):
+    """``ssw_kv_pool``."""
+    _fields_ = [("codes", _c_p), ("scales", _c_p), ("codes_layer_stride", _i64),
+                ("scales_layer_stride", _i64), ("codes_page_stride", _i64),
+                ("scales_page_stride", _i64), ("codes_page_bytes", _i64),
+                ("scales_page_bytes", _i64), ("num_pages", _i64), ("layers", ctypes.c_int32)]
 
 
 ABI_VERSION = 1

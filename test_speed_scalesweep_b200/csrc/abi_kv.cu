@@ -262,4 +262,187 @@ int ssw_nvfp4_paged_attention(const ssw_kv_cache* cache, const ssw_kv_attention*
   return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
 }
 
+namespace {
+
+int check_pool(const char* name, const ssw_kv_pool* p, ssw::kv::PoolArgs* out) {
+  if (!p) return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null pool", name);
+  if (p->layers < 1 || p->num_pages < 1 || p->num_pages >= (1ll << 31))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad sizes layers=%d num_pages=%lld", name, p->layers,
+                (long long)p->num_pages);
+  if (p->codes_page_bytes < 16 || p->scales_page_bytes < 16 || p->codes_page_bytes % 16 ||
+      p->scales_page_bytes % 16 || p->codes_page_bytes > (1ll << 30) ||
+      p->scales_page_bytes > (1ll << 30))
+    return fail(SSW_ERR_INVALID_ARGUMENT,
+                "%s: a page's bytes must be a multiple of 16 up to 2^30 (got %lld and %lld)", name,
+                (long long)p->codes_page_bytes, (long long)p->scales_page_bytes);
+  if (p->codes_page_stride % 16 || p->scales_page_stride % 16 || p->codes_layer_stride % 16 ||
+      p->scales_layer_stride % 16 || p->codes_page_stride < p->codes_page_bytes ||
+      p->scales_page_stride < p->scales_page_bytes)
+    return fail(SSW_ERR_INVALID_ARGUMENT,
+                "%s: strides must be multiples of 16 bytes and pages must not overlap", name);
+  if (!p->codes || !p->scales || !aligned(p->codes, 16) || !aligned(p->scales, 16))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: codes and scales must be 16-byte aligned, not null",
+                name);
+  out->codes = p->codes;
+  out->scales = p->scales;
+  out->codes_layer_stride = p->codes_layer_stride;
+  out->scales_layer_stride = p->scales_layer_stride;
+  out->codes_page_stride = p->codes_page_stride;
+  out->scales_page_stride = p->scales_page_stride;
+  out->codes_page_bytes = p->codes_page_bytes;
+  out->scales_page_bytes = p->scales_page_bytes;
+  out->num_pages = p->num_pages;
+  out->layers = p->layers;
+  return SSW_OK;
+}
+
+int check_pages(const char* name, const ssw_kv_pages* t, int64_t n, const int32_t* seqs,
+                const int32_t* other, bool two, ssw::kv::PagesArgs* a) {
+  if (!t) return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null page tables", name);
+  if (t->page_size != 16 && t->page_size != 32 && t->page_size != 64 && t->page_size != 128)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: page_size must be 16, 32, 64 or 128 (got %d)", name,
+                t->page_size);
+  if (t->num_pages < 1 || t->num_pages > (1 << 30) || t->max_seqs < 1 || t->columns < 1 ||
+      t->table_stride < t->columns)
+    return fail(SSW_ERR_INVALID_ARGUMENT,
+                "%s: bad sizes num_pages=%d max_seqs=%d columns=%d stride=%lld", name, t->num_pages,
+                t->max_seqs, t->columns, (long long)t->table_stride);
+  if (n < 0 || n > t->max_seqs)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: %lld sequences named, the table has %d", name,
+                (long long)n, t->max_seqs);
+  if (!t->refcount || !t->block_table || !t->seq_lens || (n > 0 && (!seqs || (two && !other))))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  if (!aligned(t->refcount, 4) || !aligned(t->block_table, 4) || !aligned(t->seq_lens, 4) ||
+      !aligned(t->status, 4) || !aligned(seqs, 4) || !aligned(other, 4))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: misaligned pointer", name);
+  a->refcount = t->refcount;
+  a->block_table = t->block_table;
+  a->table_stride = t->table_stride;
+  a->seq_lens = t->seq_lens;
+  a->status = t->status;
+  a->num_pages = t->num_pages;
+  a->max_seqs = t->max_seqs;
+  a->columns = t->columns;
+  a->page_shift = 4;
+  while ((1 << a->page_shift) < t->page_size) ++a->page_shift;
+  a->seqs = seqs;
+  a->other = other;
+  a->n = (int32_t)n;
+  return SSW_OK;
+}
+
+int check_workspace(const char* name, void* workspace, int64_t have, int64_t words) {
+  if (!workspace || !aligned(workspace, 4) || have < words * 4)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: the workspace must hold %lld bytes", name,
+                (long long)(words * 4));
+  return SSW_OK;
+}
+
+int64_t most_new_pages(int64_t n, int64_t tokens, int page_size) { return n + tokens / page_size; }
+
+}  // namespace
+
+int64_t ssw_kv_pages_workspace_bytes(int64_t n, int64_t total_tokens, int page_size,
+                                     int64_t num_pages) {
+  if (n < 0 || total_tokens < 0 || page_size < 1 || num_pages < 0) return -1;
+  const int64_t pages = most_new_pages(n, total_tokens, page_size);
+  return 4 * ssw::kv::pages_workspace_words(n, pages > num_pages ? pages : num_pages, num_pages);
+}
+
+int ssw_kv_pages_fork(const ssw_kv_pages* tables, const ssw_kv_pool* pool, int64_t n,
+                      const int32_t* parents, const int32_t* children, void* workspace,
+                      int64_t workspace_bytes, void* stream) {
+  const char* name = "kv_pages_fork";
+  ssw::set_last_error("");
+  ssw::kv::PagesArgs a;
+  ssw::kv::PoolArgs c;
+  int st = check_pages(name, tables, n, parents, children, true, &a);
+  if (st == SSW_OK) st = check_pool(name, pool, &c);
+  if (st != SSW_OK) return st;
+  if (pool->num_pages != tables->num_pages)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: the pool has %lld pages, the tables %d", name,
+                (long long)pool->num_pages, tables->num_pages);
+  if (n == 0) return SSW_OK;
+  st = check_workspace(name, workspace, workspace_bytes, ssw::kv::pages_workspace_words(n, n, 0));
+  if (st != SSW_OK) return st;
+  const int sms = device_sms();
+  if (sms < 0) return fail(SSW_ERR_CUDA, "%s: no CUDA device", name);
+  const cudaError_t e = ssw::kv::launch_fork(a, c, static_cast<int32_t*>(workspace), sms,
+                                             static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
+}
+
+int ssw_kv_pages_free(const ssw_kv_pages* tables, int64_t n, const int32_t* seqs, void* stream) {
+  const char* name = "kv_pages_free";
+  ssw::set_last_error("");
+  ssw::kv::PagesArgs a;
+  int st = check_pages(name, tables, n, seqs, nullptr, false, &a);
+  if (st != SSW_OK || n == 0) return st;
+  const cudaError_t e = ssw::kv::launch_free(a, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
+}
+
+int ssw_kv_pages_extend(const ssw_kv_pages* tables, int64_t n, const int32_t* seqs,
+                        const int32_t* new_tokens, int64_t total_tokens, int64_t* slot_mapping,
+                        void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* name = "kv_pages_extend";
+  ssw::set_last_error("");
+  ssw::kv::PagesArgs a;
+  int st = check_pages(name, tables, n, seqs, new_tokens, true, &a);
+  if (st != SSW_OK) return st;
+  if (total_tokens < 0 || total_tokens >= (1ll << 30) || (n == 0 && total_tokens > 0))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad number of new tokens (%lld)", name,
+                (long long)total_tokens);
+  if (n == 0) return SSW_OK;
+  if (total_tokens > 0 && (!slot_mapping || !aligned(slot_mapping, 8)))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null or misaligned slot_mapping", name);
+  const int64_t most = most_new_pages(n, total_tokens, tables->page_size);
+  st = check_workspace(name, workspace, workspace_bytes, ssw::kv::pages_workspace_words(n, most, 0));
+  if (st != SSW_OK) return st;
+  const cudaError_t e = ssw::kv::launch_extend(a, total_tokens, most, slot_mapping,
+                                               static_cast<int32_t*>(workspace),
+                                               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
+}
+
+int ssw_kv_pages_compact(const ssw_kv_pages* tables, const ssw_kv_pool* pool, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  const char* name = "kv_pages_compact";
+  ssw::set_last_error("");
+  ssw::kv::PagesArgs a;
+  ssw::kv::PoolArgs c;
+  int st = check_pages(name, tables, 0, nullptr, nullptr, false, &a);
+  if (st == SSW_OK) st = check_pool(name, pool, &c);
+  if (st != SSW_OK) return st;
+  if (pool->num_pages != tables->num_pages)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: the pool has %lld pages, the tables %d", name,
+                (long long)pool->num_pages, tables->num_pages);
+  st = check_workspace(name, workspace, workspace_bytes,
+                       ssw::kv::pages_workspace_words(0, tables->num_pages, tables->num_pages));
+  if (st != SSW_OK) return st;
+  const int sms = device_sms();
+  if (sms < 0) return fail(SSW_ERR_CUDA, "%s: no CUDA device", name);
+  const cudaError_t e = ssw::kv::launch_compact(a, c, static_cast<int32_t*>(workspace), sms,
+                                                static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
+}
+
+int ssw_kv_pages_copy(const ssw_kv_pool* pool, int64_t n, const int32_t* source,
+                      const int32_t* target, void* stream) {
+  const char* name = "kv_pages_copy";
+  ssw::set_last_error("");
+  ssw::kv::PoolArgs c;
+  int st = check_pool(name, pool, &c);
+  if (st != SSW_OK) return st;
+  if (n < 0 || n >= (1ll << 31)) return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad size", name);
+  if (n == 0) return SSW_OK;
+  if (!source || !target || !aligned(source, 4) || !aligned(target, 4))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null or misaligned page list", name);
+  const int sms = device_sms();
+  if (sms < 0) return fail(SSW_ERR_CUDA, "%s: no CUDA device", name);
+  const cudaError_t e = ssw::kv::launch_copy(c, source, target, n, sms,
+                                             static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? SSW_OK : cuda_fail(e, name);
+}
+
 }  // extern "C"

@@ -79,5 +79,43 @@ struct AttendArgs {
 int64_t attend_workspace_bytes(const AttendArgs& a, int device_sms);
 cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stream);
 
+enum { kPagesExhausted = 1, kPagesBadIndex = 2, kPagesTooLong = 3 };
+
+// The page tables of a cache and one request list.
+struct PagesArgs {
+  int32_t* refcount;     // [num_pages]
+  int32_t* block_table;  // [max_seqs, columns]
+  int64_t table_stride;  // elements
+  int32_t* seq_lens;     // [max_seqs]
+  int32_t* status;       // or null
+  int32_t num_pages, max_seqs, columns, page_shift;
+  const int32_t* seqs;   // [n]: parents, or sequences
+  const int32_t* other;  // [n]: children, or numbers of new tokens
+  int32_t n;
+};
+
+// The bytes of a cache's pages, over all its layers.
+struct PoolArgs {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t codes_layer_stride, scales_layer_stride;  // bytes
+  int64_t codes_page_stride, scales_page_stride;
+  int64_t codes_page_bytes, scales_page_bytes;      // multiples of 16
+  int64_t num_pages;
+  int32_t layers;
+  int32_t code_chunks, scale_chunks;                // filled at launch
+};
+
+int64_t pages_workspace_words(int64_t n, int64_t pages, int64_t num_pages_for_remap);
+cudaError_t launch_fork(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, int device_sms,
+                        cudaStream_t stream);
+cudaError_t launch_free(const PagesArgs& a, cudaStream_t stream);
+cudaError_t launch_extend(const PagesArgs& a, int64_t total_tokens, int64_t most_pages,
+                          int64_t* slots, int32_t* ws, cudaStream_t stream);
+cudaError_t launch_compact(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, int device_sms,
+                           cudaStream_t stream);
+cudaError_t launch_copy(const PoolArgs& pool, const int32_t* source, const int32_t* target,
+                        int64_t pairs, int device_sms, cudaStream_t stream);
+
 }  // namespace kv
 }  // namespace ssw

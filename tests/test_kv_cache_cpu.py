@@ -150,3 +150,59 @@ def test_attention_refusals(built_library, kw, needle):
 
 def test_attention_of_nothing_is_a_no_op(built_library):
     assert attention(tokens=0) == 0 and attention(seqs=0) == 0
+
+
+def tables(**kw):
+    d = dict(refcount=0x1000, block_table=0x2000, table_stride=4, seq_lens=0x3000, status=None,
+             num_pages=8, max_seqs=4, columns=4, page_size=16)
+    d.update(kw)
+    return _lib.KVPages(**d)
+
+
+def pool(**kw):
+    d = dict(codes=0x10000, scales=0x20000, codes_layer_stride=1 << 16, scales_layer_stride=1 << 13,
+             codes_page_stride=4096, scales_page_stride=512, codes_page_bytes=4096, scales_page_bytes=512,
+             num_pages=8, layers=2)
+    d.update(kw)
+    return _lib.KVPool(**d)
+
+
+WS = (0x40000, 1 << 20, None)
+
+
+@pytest.mark.parametrize("call,needle", [
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables(page_size=8)), 1, 0x100, None), "page_size"),
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables(table_stride=3)), 1, 0x100, None), "bad sizes"),
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables()), 5, 0x100, None), "has 4"),
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables()), 1, None, None), "null"),
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables(refcount=None)), 1, 0x100, None), "null"),
+    (lambda h: h.ssw_kv_pages_free(ctypes.byref(tables()), 1, 0x102, None), "misaligned"),
+    (lambda h: h.ssw_kv_pages_fork(ctypes.byref(tables()), ctypes.byref(pool(num_pages=9)), 1, 0x100, 0x200, *WS), "the tables 8"),
+    (lambda h: h.ssw_kv_pages_fork(ctypes.byref(tables()), ctypes.byref(pool(codes_page_bytes=24)), 1, 0x100, 0x200, *WS), "multiple of 16"),
+    (lambda h: h.ssw_kv_pages_fork(ctypes.byref(tables()), ctypes.byref(pool(scales_page_stride=496)), 1, 0x100, 0x200, *WS), "overlap"),
+    (lambda h: h.ssw_kv_pages_fork(ctypes.byref(tables()), ctypes.byref(pool(layers=0)), 1, 0x100, 0x200, *WS), "layers"),
+    (lambda h: h.ssw_kv_pages_fork(ctypes.byref(tables()), ctypes.byref(pool()), 1, 0x100, 0x200, 0x40000, 8, None), "workspace"),
+    (lambda h: h.ssw_kv_pages_extend(ctypes.byref(tables()), 1, 0x100, 0x200, -1, 0x300, *WS), "new tokens"),
+    (lambda h: h.ssw_kv_pages_extend(ctypes.byref(tables()), 0, None, None, 1, 0x300, *WS), "new tokens"),
+    (lambda h: h.ssw_kv_pages_extend(ctypes.byref(tables()), 1, 0x100, 0x200, 1, None, *WS), "slot_mapping"),
+    (lambda h: h.ssw_kv_pages_extend(ctypes.byref(tables()), 1, 0x100, 0x200, 1, 0x300, None, 0, None), "workspace"),
+    (lambda h: h.ssw_kv_pages_compact(ctypes.byref(tables()), ctypes.byref(pool()), 0x40002, 1 << 20, None), "workspace"),
+    (lambda h: h.ssw_kv_pages_compact(ctypes.byref(tables()), ctypes.byref(pool(codes=None)), *WS), "null"),
+    (lambda h: h.ssw_kv_pages_copy(ctypes.byref(pool()), -1, 0x100, 0x200, None), "bad size"),
+    (lambda h: h.ssw_kv_pages_copy(ctypes.byref(pool()), 1, 0x100, None, None), "null")])
+def test_pages_refusals(built_library, call, needle):
+    st = call(_lib.lib())
+    assert st == _lib.SSW_ERR_INVALID_ARGUMENT
+    with pytest.raises(ValueError, match=needle):
+        _lib.check(st)
+
+
+def test_pages_python_refusals():
+    from test_speed_scalesweep_b200 import kv_pages
+    codes, scales = kv_cache.alloc_kv_cache(4, 16, 1, 64, device="cpu", num_layers=2)
+    with pytest.raises(ValueError, match="CUDA"):
+        kv_pages.NVFP4KVPages.empty(codes, scales, 2, 2)
+    with pytest.raises(ValueError, match="layers"):
+        kv_pages.NVFP4KVPages.empty(codes[0, 0], scales[0, 0], 2, 2)
+    with pytest.raises(ValueError, match="head_size/16"):
+        kv_pages.NVFP4KVPages.empty(codes, scales[..., :2], 2, 2)
