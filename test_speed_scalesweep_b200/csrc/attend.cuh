@@ -1,0 +1,166 @@
+// What the attention kernels share: launch parameters, the rows and keys of a
+// tile, waits, copies and the exact conversions of codes and scales to f16.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "kv.cuh"
+#include "quant.cuh"
+
+namespace ssw {
+namespace kv {
+
+constexpr int kKeys = 32;        // keys of a decode stage; splits begin at multiples of it
+constexpr float kShift = 10.f;  // log2 of the scale of P
+constexpr float kSlack = 5.f;   // the maximum may grow by 2^kSlack before O is rescaled
+constexpr uint32_t kWaitLimit = 1u << 22;  // bounded spin
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+
+struct Params {
+  AttendArgs a;
+  int group;       // query heads of a kv head
+  int tiles;       // row tiles of the longest query
+  int min_rows, max_rows;  // sequences with other numbers of rows are another kernel's
+  int splits;      // CTAs that share a tile's keys
+  int chunk;       // keys of a split, a multiple of 128
+  int page_shift;
+  float* part_o;   // [split][row of q and head][head_size]
+  float* part_ml;  // [split][row of q and head][2]
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+// Bounded wait for the phase with the given parity; false = gave up.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Two f16 from one byte of codes (element 0 in the low nibble).
+__device__ __forceinline__ uint32_t e2m1_h2(uint32_t word, int byte) {
+  uint32_t r;
+  const uint16_t b = (uint16_t)((word >> (8 * byte)) & 0xFF);
+  asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}"
+      : "=r"(r)
+      : "h"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_h2(uint32_t two) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The rows and keys of one tile.
+struct Tile {
+  int row0, rows;        // first of the sequence's rows, rows here
+  int first_token;       // global token of the sequence's token 0
+  int offset;            // position of the sequence's token 0
+  int beg, end;          // keys that any of its rows sees
+  int all_beg, all_end;  // keys that all of its rows see
+};
+
+__device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int tile_rows,
+                                        Tile& t) {
+  const AttendArgs& a = p.a;
+  const int q0 = a.query_start[seq];
+  int len = a.query_start[seq + 1] - q0;
+  if (q0 < 0 || len <= 0) return false;
+  const int kv = max(0, a.seq_lens[seq]);
+  t.offset = kv - len;
+  if (q0 >= a.tokens) return false;
+  if (len > a.tokens - q0) len = (int)(a.tokens - q0);
+  const int64_t rows64 = (int64_t)len * p.group;
+  if (rows64 < p.min_rows || rows64 > p.max_rows) return false;
+  const int rows = (int)rows64;
+  t.row0 = tile * tile_rows;
+  if (t.row0 >= rows) return false;
+  t.rows = min(tile_rows, rows - t.row0);
+  t.first_token = q0;
+  const int lo = t.offset + t.row0 / p.group;
+  const int hi = t.offset + (t.row0 + t.rows - 1) / p.group;
+  const int room = (int)min((int64_t)a.table_columns << p.page_shift, (int64_t)kv);
+  t.end = a.causal ? min(room, hi + 1) : room;
+  t.all_end = a.causal ? min(room, lo + 1) : room;
+  t.beg = a.window >= 0 ? max(0, lo - a.window) : 0;
+  t.all_beg = a.window >= 0 ? max(0, hi - a.window) : 0;
+  t.end = max(t.end, 0);
+  return true;
+}
+
+// Splits of a tile that hold keys (at least one, which then writes zeros).
+__device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
+  const int n = t.end - (t.beg & ~(kKeys - 1));
+  return max(1, (n + p.chunk - 1) / p.chunk);
+}
+
+__device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype) {  // 2 values
+  if (dtype == kDTypeBF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+    *reinterpret_cast<__nv_bfloat162*>(dst) = h;
+  } else {
+    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(v[0], v[1]);
+  }
+}
+
+// Tiles of 256 rows on the tensor cores' own memory (kv_prompt.cu); head sizes 64 and 128.
+constexpr int kPromptRows = 256;
+cudaError_t launch_prompt(const Params& p, cudaStream_t stream);
+
+}  // namespace kv
+}  // namespace ssw

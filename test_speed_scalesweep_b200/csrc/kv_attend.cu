@@ -30,6 +30,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "attend.cuh"
 #include "kv.cuh"
 #include "quant.cuh"
 
@@ -39,138 +40,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kKeys = 32;      // keys of a stage
-constexpr float kShift = 10.f;  // log2 of the scale of P
-constexpr float kSlack = 5.f;   // the maximum may grow by 2^kSlack before O is rescaled
-constexpr uint32_t kWaitLimit = 1u << 22;  // bounded spin
-constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
-
-struct Params {
-  AttendArgs a;
-  int group;       // query heads of a kv head
-  int tiles;       // row tiles of the longest query
-  int splits;      // CTAs that share a tile's keys
-  int chunk;       // keys of a split, a multiple of kKeys * kWarps
-  int page_shift;
-  float* part_o;   // [split][row of q and head][head_size]
-  float* part_ml;  // [split][row of q and head][2]
-};
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-// Bounded wait for the phase with the given parity; false = gave up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(dst),
-      "l"(src), "r"(bytes), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// Two f16 from one byte of codes (element 0 in the low nibble).
-__device__ __forceinline__ uint32_t e2m1_h2(uint32_t word, int byte) {
-  uint32_t r;
-  const uint16_t b = (uint16_t)((word >> (8 * byte)) & 0xFF);
-  asm("{\n\t.reg .b8 lo, hi;\n\tmov.b16 {lo, hi}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, lo;\n\t}"
-      : "=r"(r)
-      : "h"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3_h2(uint32_t two) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two));
-  return r;
-}
-__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
-  uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The rows and keys of one tile.
-struct Tile {
-  int row0, rows;        // first of the sequence's rows, rows here
-  int first_token;       // global token of the sequence's token 0
-  int offset;            // position of the sequence's token 0
-  int beg, end;          // keys that any of its rows sees
-  int all_beg, all_end;  // keys that all of its rows see
-};
-
-__device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int tile_rows,
-                                        Tile& t) {
-  const AttendArgs& a = p.a;
-  const int q0 = a.query_start[seq];
-  int len = a.query_start[seq + 1] - q0;
-  if (q0 < 0 || len <= 0) return false;
-  const int kv = max(0, a.seq_lens[seq]);
-  t.offset = kv - len;
-  if (q0 >= a.tokens) return false;
-  if (len > a.tokens - q0) len = (int)(a.tokens - q0);
-  const int rows = len * p.group;
-  t.row0 = tile * tile_rows;
-  if (t.row0 >= rows) return false;
-  t.rows = min(tile_rows, rows - t.row0);
-  t.first_token = q0;
-  const int lo = t.offset + t.row0 / p.group;
-  const int hi = t.offset + (t.row0 + t.rows - 1) / p.group;
-  const int room = (int)min((int64_t)a.table_columns << p.page_shift, (int64_t)kv);
-  t.end = a.causal ? min(room, hi + 1) : room;
-  t.all_end = a.causal ? min(room, lo + 1) : room;
-  t.beg = a.window >= 0 ? max(0, lo - a.window) : 0;
-  t.all_beg = a.window >= 0 ? max(0, hi - a.window) : 0;
-  t.end = max(t.end, 0);
-  return true;
-}
-
-// Splits of a tile that hold keys (at least one, which then writes zeros).
-__device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
-  const int n = t.end - (t.beg & ~(kKeys - 1));
-  return max(1, (n + p.chunk - 1) / p.chunk);
-}
 
 template <int kD>
 struct Shape {
@@ -189,15 +58,6 @@ constexpr int smem_bytes() {
   constexpr int ring = kWarps * Shape<kD>::kRing;
   constexpr int merge = kWarps * kNT * 8 * (kD + 2) * 4;
   return (ring > merge ? ring : merge) + kWarps * Shape<kD>::kStages * 8;
-}
-
-__device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype) {  // 2 values
-  if (dtype == kDTypeBF16) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
-    *reinterpret_cast<__nv_bfloat162*>(dst) = h;
-  } else {
-    *reinterpret_cast<__half2*>(dst) = __floats2half2_rn(v[0], v[1]);
-  }
 }
 
 template <int kD, int kNT>
@@ -646,35 +506,65 @@ int log2i(int v) {
   return s;
 }
 
-struct Plan {
-  int rows;  // of a tile
+// How one kernel cuts the batch.
+struct Cut {
+  int rows;  // of a tile; 0: not launched
   int tiles, splits, chunk;
+  int min_rows, max_rows;
+};
+struct Plan {
+  Cut decode, prompt;
 };
 
+// `most` rows at most per sequence; `target` CTAs keep the GPU busy evenly.
+Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int64_t min_chunk) {
+  Cut c;
+  c.rows = tile_rows;
+  c.tiles = (int)((most + tile_rows - 1) / tile_rows);
+  const int group = a.q_heads / a.cache.kv_heads;
+  const int64_t tokens = (tile_rows + group - 1) / group + 1;  // that a tile's rows touch
+  int64_t span = a.max_seq_len;
+  if (a.window >= 0 && span > (int64_t)a.window + tokens + kKeys)
+    span = (int64_t)a.window + tokens + kKeys;
+  const int64_t units = (int64_t)a.seqs * c.tiles * a.cache.kv_heads;
+  const int64_t splits = target / units < 1 ? 1 : target / units;
+  int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
+  if (chunk < min_chunk) chunk = min_chunk;
+  c.chunk = (int)chunk;
+  // the first key of a windowed tile is rounded down to a stage
+  c.splits = (int)((span + (a.window >= 0 ? kKeys - 1 : 0) + chunk - 1) / chunk);
+  return c;
+}
+
 Plan plan_of(const AttendArgs& a, int device_sms) {
-  Plan pl;
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t rows = (int64_t)a.max_query_len * group;
-  pl.rows = rows <= 8 ? 8 : rows <= 16 || a.cache.head_size == 256 ? 16 : 32;
-  pl.tiles = (int)((rows + pl.rows - 1) / pl.rows);
-  int64_t span = a.max_seq_len;
-  if (a.window >= 0 && span > (int64_t)a.window + a.max_query_len + kKeys)
-    span = (int64_t)a.window + a.max_query_len + kKeys;
-  const int64_t units = (int64_t)a.seqs * pl.tiles * a.cache.kv_heads;
-  const int64_t want = (int64_t)device_sms * 3 * 4;
-  int64_t splits = (want + units - 1) / units;
-  constexpr int kStep = kKeys * kWarps;
-  int64_t chunk = ((span + splits - 1) / splits + kStep - 1) / kStep * kStep;
-  if (chunk < 2 * kStep) chunk = 2 * kStep;
-  pl.chunk = (int)chunk;
-  // the first key of a windowed tile is rounded down to a stage
-  pl.splits = (int)((span + kKeys - 1 + chunk - 1) / chunk);
-  if (pl.splits < 1) pl.splits = 1;
+  const int most = a.cache.head_size == 256 ? 16 : 32;  // rows of decode_kernel's largest tile
+  Plan pl = {};
+  if (rows <= most || a.cache.head_size == 256) {
+    pl.decode = cut_of(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, (int64_t)device_sms * 12, 256);
+    pl.decode.max_rows = 0x7FFFFFFF;
+    return pl;
+  }
+  pl.prompt = cut_of(a, kPromptRows, rows, device_sms, 512);
+  pl.prompt.max_rows = 0x7FFFFFFF;
+  if (a.seqs > 1) {  // single tokens among prompts
+    pl.decode = cut_of(a, group <= 8 ? 8 : 16, 16, (int64_t)device_sms * 12, 256);
+    pl.decode.max_rows = pl.decode.rows;
+    pl.decode.tiles = 1;
+    pl.prompt.min_rows = pl.decode.rows + 1;
+  }
   return pl;
 }
 
+int most_splits(const Plan& pl) {
+  const int a = pl.decode.rows ? pl.decode.splits : 1, b = pl.prompt.rows ? pl.prompt.splits : 1;
+  return a > b ? a : b;
+}
+
 int64_t part_rows(const AttendArgs& a, const Plan& pl) {
-  return pl.splits > 1 ? (int64_t)pl.splits * a.tokens * a.q_heads : 0;
+  const int splits = most_splits(pl);
+  return splits > 1 ? (int64_t)splits * a.tokens * a.q_heads : 0;
 }
 
 template <int kD, int kNT>
@@ -686,10 +576,6 @@ cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
   decode_kernel<kD, kNT><<<grid, kThreads, kSmem, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess || p.splits == 1) return e;
-  const dim3 jgrid(grid.x, kNT * 8 / kWarps, grid.z);
-  join_kernel<kD><<<jgrid, kThreads, 0, stream>>>(p, kNT * 8);
   return cudaGetLastError();
 }
 
@@ -701,27 +587,44 @@ cudaError_t launch_rows(const Params& p, int rows, cudaStream_t stream) {
   return cudaErrorInvalidValue;
 }
 
+cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
+  if (c.rows == 0) return cudaSuccess;
+  p.tiles = c.tiles;
+  p.splits = c.splits;
+  p.chunk = c.chunk;
+  p.min_rows = c.min_rows;
+  p.max_rows = c.max_rows;
+  const int d = p.a.cache.head_size;
+  cudaError_t e = c.rows == kPromptRows ? launch_prompt(p, stream)
+                  : d == 64             ? launch_rows<64>(p, c.rows, stream)
+                  : d == 128            ? launch_rows<128>(p, c.rows, stream)
+                                        : launch_rows<256>(p, c.rows, stream);
+  if (e != cudaSuccess || c.splits == 1) return e;
+  const dim3 grid((unsigned)(p.a.seqs * p.tiles), (c.rows + kWarps - 1) / kWarps,
+                  p.a.cache.kv_heads);
+  if (d == 64) join_kernel<64><<<grid, kThreads, 0, stream>>>(p, c.rows);
+  else if (d == 128) join_kernel<128><<<grid, kThreads, 0, stream>>>(p, c.rows);
+  else join_kernel<256><<<grid, kThreads, 0, stream>>>(p, c.rows);
+  return cudaGetLastError();
+}
+
 }  // namespace
 
 int64_t attend_workspace_bytes(const AttendArgs& a, int device_sms) {
-  const Plan pl = plan_of(a, device_sms);
-  return part_rows(a, pl) * (a.cache.head_size + 2) * (int64_t)sizeof(float);
+  return part_rows(a, plan_of(a, device_sms)) * (a.cache.head_size + 2) * (int64_t)sizeof(float);
 }
 
 cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stream) {
   const Plan pl = plan_of(a, device_sms);
-  Params p;
+  Params p = {};
   p.a = a;
+  if (a.window > (1 << 30)) p.a.window = 1 << 30;  // positions stay below it
   p.group = a.q_heads / a.cache.kv_heads;
-  p.tiles = pl.tiles;
-  p.splits = pl.splits;
-  p.chunk = pl.chunk;
   p.page_shift = log2i(a.cache.page_size);
   p.part_o = a.workspace;
   p.part_ml = a.workspace ? a.workspace + part_rows(a, pl) * a.cache.head_size : nullptr;
-  if (a.cache.head_size == 64) return launch_rows<64>(p, pl.rows, stream);
-  if (a.cache.head_size == 128) return launch_rows<128>(p, pl.rows, stream);
-  return launch_rows<256>(p, pl.rows, stream);
+  const cudaError_t e = launch_cut(p, pl.prompt, stream);
+  return e != cudaSuccess ? e : launch_cut(p, pl.decode, stream);
 }
 
 }  // namespace kv

@@ -1,0 +1,541 @@
+// Attention over an NVFP4 cache for long queries (see kv_attend.cu for the
+// operator): tiles of 256 (token, head) rows of one kv head, 128 keys a block,
+// on the 5th-generation tensor cores.
+//
+//   S = Q K^T  (tcgen05.mma kind::f16, Q and K from shared memory, S in TMEM)
+//   P = 2^(scale S - m + kShift)  (f16, written over S in TMEM)
+//   O += P V   (P from TMEM, V from shared memory, O in TMEM)
+//
+// One CTA per SM.  The two 128-row halves of a tile take turns: while the
+// tensor cores work on one half's P V and next Q K^T, a warpgroup forms the
+// other half's softmax.  Warps:
+//   0-3, 4-7  softmax of half 0 / 1, one row per thread; also Q's load and the
+//             result's store
+//   8-11      dequantization: thread i turns key i of a block from codes and
+//             scales (prefetched one block ahead in registers) into f16 rows,
+//             once for all 256 rows, in a ring of four tiles (K, V, K, V)
+//   12        issues the MMAs.  It meets the others on hardware named barriers
+//             only: a shared-memory access by the issuing warp would wait for
+//             its queued MMAs to drain.
+// A row's O is rescaled only when its maximum grows by more than 2^kSlack
+// (P keeps that much room below f16's largest), so almost never after the first
+// blocks, and by the softmax threads: the P V before it has completed when the
+// next S has (MMAs complete in order), and the next one waits for this P.
+//
+// Every mbarrier wait is bounded; after one that gave up the roles keep their
+// barrier protocol, so no partner is left waiting, and *status is set.
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "attend.cuh"
+#include "kv.cuh"
+#include "quant.cuh"
+
+namespace ssw {
+namespace kv {
+namespace {
+
+constexpr int kPThreads = 13 * 32;
+constexpr int kBlock = 128;  // keys of a block
+constexpr int kWarpDequant = 8, kWarpMma = 12;
+constexpr int kMaskRing = 4;
+
+// Named barriers: tile slots 1..4 full, P of half 0 / 1, Q loaded.
+constexpr int kBarSlot = 1, kBarP = 5, kBarQ = 7;
+
+template <int kD>
+struct PromptShape {
+  static constexpr int kHalf = 128 * 128;             // bytes: 128 rows x 64 f16
+  static constexpr int kTile = kHalf * (kD / 64);     // 128 rows x kD f16
+  static constexpr int kSmem = 2 * kTile + 4 * kTile + 256 + 1024;
+  static constexpr uint32_t kS = 0, kO = 256;         // TMEM columns: S0, S1, then O0, O1
+  static constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kBlock >> 3) << 17) | (8u << 24);
+  // B (V) is contiguous along N
+  static constexpr uint32_t kIdescPV =
+      (1u << 4) | (1u << 16) | ((uint32_t)(kD >> 3) << 17) | (8u << 24);
+};
+
+struct Control {
+  uint64_t empty[4];
+  uint64_t s_full[2];
+  uint64_t mask_full[kMaskRing];
+  uint32_t mask[kMaskRing][4];  // bit i: key i of the block is there
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+      : "memory");
+}
+// Shared-memory matrix descriptor: 128-byte swizzle, version 1.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)((lbo >> 4) & 0x3FFF) << 16) |
+         ((uint64_t)((sbo >> 4) & 0x3FFF) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+// 32 columns of the warp's 32 lanes; the caller waits with tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, "
+      "%10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
+      "%26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+        "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+        "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]),
+        "=r"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
+      "%28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                            uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+// Byte offset of 16-byte chunk c of row r in a 128-row tile of 64-wide halves,
+// 128-byte swizzle: K-major for Q and K, N-major for V.
+__device__ __forceinline__ uint32_t tile_offset(int r, int c) {
+  return (uint32_t)((c >> 3) * 16384 + (r >> 3) * 1024 + (r & 7) * 128 + (((c ^ r) & 7) << 4));
+}
+
+// Codes and scales of one key or value row.
+template <int kD>
+struct RowRegs {
+  uint32_t codes[kD / 8];
+  uint32_t scales[kD / 64];
+};
+
+template <int kD>
+__device__ __forceinline__ void load_row(RowRegs<kD>& r, const uint8_t* codes,
+                                         const uint8_t* scales, bool there) {
+  if (there) {
+#pragma unroll
+    for (int j = 0; j < kD / 32; ++j)
+      *reinterpret_cast<uint4*>(&r.codes[4 * j]) = __ldg(reinterpret_cast<const uint4*>(codes) + j);
+    if constexpr (kD == 64) {
+      r.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(scales));
+    } else {
+      *reinterpret_cast<uint2*>(r.scales) = __ldg(reinterpret_cast<const uint2*>(scales));
+    }
+  } else {  // what lies behind the last key may hold anything, NaN scales too
+#pragma unroll
+    for (int j = 0; j < kD / 8; ++j) r.codes[j] = 0;
+#pragma unroll
+    for (int j = 0; j < kD / 64; ++j) r.scales[j] = 0;
+  }
+}
+
+template <int kD>
+__device__ __forceinline__ void store_row(const RowRegs<kD>& r, uint32_t tile, int row) {
+#pragma unroll
+  for (int b = 0; b < kD / 16; ++b) {
+    const uint32_t two = e4m3_h2(r.scales[b / 4] >> (16 * ((b / 2) & 1)));
+    const uint32_t f = __byte_perm(two, two, b & 1 ? 0x3232 : 0x1010);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t w = r.codes[2 * b + h];
+      st_shared16(tile + tile_offset(row, 2 * b + h), mul_h2(e2m1_h2(w, 0), f),
+                  mul_h2(e2m1_h2(w, 1), f), mul_h2(e2m1_h2(w, 2), f), mul_h2(e2m1_h2(w, 3), f));
+    }
+  }
+}
+
+template <int kD>
+__global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
+  using S = PromptShape<kD>;
+  extern __shared__ uint8_t smem_raw[];
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
+  // the last tiles see the most keys: they start first
+  Tile tile;
+  if (!tile_of(p, seq, p.tiles - 1 - blockIdx.x % p.tiles, kPromptRows, tile)) return;
+  const int base = tile.beg & ~(kKeys - 1);
+  if (split > 0 && base + (int64_t)split * p.chunk >= tile.end) return;
+  const int c0 = base + split * p.chunk;
+  const int c1 = (int)min((int64_t)tile.end, (int64_t)c0 + p.chunk);
+  const int blocks = c1 > c0 ? (c1 - c0 + kBlock - 1) / kBlock : 0;
+  const bool two = tile.rows > 128;
+
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t q_tile = smem, ring = smem + 2 * S::kTile;
+  Control* ctl =
+      reinterpret_cast<Control*>(smem_raw + (ring + 4 * S::kTile - smem_u32(smem_raw)));
+  static_assert(sizeof(Control) <= 256, "control block");
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&ctl->empty[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctl->s_full[i]), 1);
+    for (int i = 0; i < kMaskRing; ++i) mbar_init(smem_u32(&ctl->mask_full[i]), 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&ctl->tmem)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
+  bool ok = true;
+
+  if (warp == kWarpMma) {
+    bar_sync(kBarQ, 256 + 32);
+    auto qk = [&](int half, int slot) {
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < kD / 16; ++j) {
+          const uint32_t off = (j / 4) * S::kHalf + 32 * (j % 4);
+          mma_ss(tmem + S::kS + 128 * half, smem_desc(q_tile + half * S::kTile + off, 16, 1024),
+                 smem_desc(ring + slot * S::kTile + off, 16, 1024), S::kIdescQK, j != 0);
+        }
+        mma_commit(smem_u32(&ctl->s_full[half]));
+      }
+    };
+    auto pv = [&](int half, int slot, bool first) {
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < kBlock / 16; ++j)
+          mma_ts(tmem + S::kO + kD * half, tmem + S::kS + 128 * half + 8 * j,
+                 smem_desc(ring + slot * S::kTile + 2048 * j, S::kHalf, 1024), S::kIdescPV,
+                 !(first && j == 0));
+      }
+    };
+    if (blocks > 0) {
+      bar_sync(kBarSlot, 128 + 32);
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      qk(0, 0);
+      if (two) qk(1, 0);
+      // a slot's release is committed only where it is waited for: no arrival
+      // may be in flight when the CTA ends
+      if (lane == 0 && blocks > 2) mma_commit(smem_u32(&ctl->empty[0]));
+      for (int j = 0; j < blocks; ++j) {
+        const int v_slot = (2 * j + 1) & 3, k_slot = (2 * j + 2) & 3;
+        const bool more = j + 1 < blocks;
+        bar_sync(kBarSlot + v_slot, 128 + 32);
+        if (more) bar_sync(kBarSlot + k_slot, 128 + 32);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half == 1 && !two) break;
+          bar_sync(kBarP + half, 128 + 32);
+          asm volatile("tcgen05.fence::after_thread_sync;");
+          pv(half, v_slot, j == 0);
+          if (more)
+            qk(half, k_slot);
+          else if (lane == 0)
+            mma_commit(smem_u32(&ctl->s_full[half]));  // the last P V
+        }
+        if (lane == 0 && j + 2 < blocks) mma_commit(smem_u32(&ctl->empty[v_slot]));
+        if (lane == 0 && j + 3 < blocks) mma_commit(smem_u32(&ctl->empty[k_slot]));
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kWarpDequant) {
+    const int i = threadIdx.x - kWarpDequant * 32;  // this thread's key of a block
+    const int page_mask = (1 << p.page_shift) - 1;
+    const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
+    const int64_t side = (int64_t)a.cache.kv_heads << p.page_shift;
+    auto page_of = [&](int j) -> int {
+      const int key = c0 + j * kBlock + i;
+      if (key >= c1 || key < tile.beg) return -1;
+      const int pg = __ldg(table + (key >> p.page_shift));
+      return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
+    };
+    auto fetch = [&](RowRegs<kD>& r, int j, int pg, int value) {
+      const int key = c0 + j * kBlock + i;
+      const int64_t row = value * side + ((int64_t)head << p.page_shift) + (key & page_mask);
+      load_row<kD>(r, a.cache.codes + pg * a.cache.codes_page_stride + row * (kD / 2),
+                   a.cache.scales + pg * a.cache.scales_page_stride + row * (kD / 16), pg >= 0);
+    };
+    RowRegs<kD> k, v;
+    int pg = page_of(0), pg_next = page_of(1);
+    fetch(k, 0, pg, 0);
+    fetch(v, 0, pg, 1);
+    for (int j = 0; j < blocks; ++j) {
+      const int k_slot = (2 * j) & 3, v_slot = k_slot + 1;
+      const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
+      // slots are used every second block
+      if (j >= 2 && ok) ok = mbar_wait(smem_u32(&ctl->empty[k_slot]), ((j >> 1) - 1) & 1);
+      if (lane == 0) {
+        ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
+        mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
+      }
+      store_row<kD>(k, ring + k_slot * S::kTile, i);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(kBarSlot + k_slot, 128 + 32);
+      pg = pg_next;
+      pg_next = page_of(j + 2);
+      fetch(k, j + 1, pg, 0);
+      if (j >= 2 && ok) ok = mbar_wait(smem_u32(&ctl->empty[v_slot]), ((j >> 1) - 1) & 1);
+      store_row<kD>(v, ring + v_slot * S::kTile, i);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(kBarSlot + v_slot, 128 + 32);
+      fetch(v, j + 1, pg, 1);
+    }
+  } else {
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane, row_in = half * 128 + r;
+    const bool live = row_in < tile.rows;
+    const int row = tile.row0 + row_in, token = row / p.group, qh = head * p.group + row % p.group;
+    // ---- Q: this thread's row, scaled as in decode_kernel, into the swizzled tile
+    float scale = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+    const bool flip = scale < 0.0f;  // the maximum below is taken before scaling
+    scale = fabsf(scale);
+    const uint16_t* src = a.q.p + (int64_t)(tile.first_token + token) * a.q.token_stride +
+                          (int64_t)qh * a.q.head_stride;
+    float down = 1.0f;
+    if (a.dtype == kDTypeBF16 && live) {
+      uint32_t big = 0;
+#pragma unroll 4
+      for (int j = 0; j < kD / 8; ++j) {
+        const uint4 w = *(reinterpret_cast<const uint4*>(src) + j);
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
+      }
+      const int e = (int)(big >> 23);
+      if (e >= 1 && e <= 253) {
+        down = __uint_as_float((uint32_t)(254 - e) << 23);
+        scale *= __uint_as_float((uint32_t)e << 23);
+      }
+    }
+    if (flip) down = -down;
+#pragma unroll 4
+    for (int j = 0; j < kD / 8; ++j) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (live) {
+        w = *(reinterpret_cast<const uint4*>(src) + j);
+        uint32_t* x = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (a.dtype == kDTypeBF16)
+            x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
+                           __uint_as_float(x[c] & 0xFFFF0000u) * down);
+          else if (flip)
+            x[c] ^= 0x80008000u;
+        }
+      }
+      st_shared16(q_tile + half * S::kTile + tile_offset(r, j), w.x, w.y, w.z, w.w);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    bar_arrive(kBarQ, 256 + 32);
+
+    const int pos = tile.offset + token;
+    const int hi_key = !live ? -1 : a.causal ? pos : 0x7FFFFFFF;
+    const int lo_key = a.window >= 0 ? pos - a.window : 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + S::kS + 128 * half;
+    const uint32_t o_addr = tmem + lanes + S::kO + kD * half;
+    float m = -INFINITY, l = 0.0f;
+    const bool work = half == 0 || two;
+    for (int j = 0; work && j < blocks; ++j) {
+      const int k0 = c0 + j * kBlock;
+      if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      uint32_t mask[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        mask[w] = *reinterpret_cast<volatile uint32_t*>(&ctl->mask[j % kMaskRing][w]);
+        // bits of keys lo_key .. hi_key
+        const int first = k0 + 32 * w;
+        const int lo = lo_key - first, hi = hi_key - first;
+        const uint32_t above = lo <= 0 ? 0xFFFFFFFFu : lo > 31 ? 0u : 0xFFFFFFFFu << lo;
+        const uint32_t below = hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : 0xFFFFFFFFu >> (31 - hi);
+        mask[w] &= above & below;
+      }
+      const bool masked =
+          __any_sync(0xFFFFFFFFu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu);
+      if (ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), j & 1);
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      // pass 1: the row's maximum
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32];
+        tmem_ld32(s_addr + 32 * c, v);
+        tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (!((mask[c] >> x) & 1u)) v[x] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int x = 0; x < 32; ++x) mx = fmaxf(mx, __uint_as_float(v[x]));
+      }
+      mx *= scale;
+      if (__any_sync(0xFFFFFFFFu, mx > m + kSlack)) {
+        const float mn = fmaxf(m, mx);
+        const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
+        m = mn;
+        l *= f;
+        if (j > 0) {  // nothing is in O before the first block
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t v[32];
+            tmem_ld32(o_addr + 32 * c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+            tmem_st32(o_addr + 32 * c, v);
+          }
+        }
+      }
+      // pass 2: the weights
+      const float ms = m == -INFINITY ? 0.0f : m - kShift;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t v[32], w[16];
+        tmem_ld32(s_addr + 32 * c, v);
+        tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (!((mask[c] >> x) & 1u)) v[x] = 0xFF800000u;
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const float p0 = ex2(fmaf(__uint_as_float(v[2 * x]), scale, -ms));
+          const float p1 = ex2(fmaf(__uint_as_float(v[2 * x + 1]), scale, -ms));
+          sum[(2 * x) & 3] += p0;
+          sum[(2 * x + 1) & 3] += p1;
+          w[x] = pack_h2(p0, p1);
+        }
+        tmem_st16(s_addr + 16 * c, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;");
+      bar_arrive(kBarP + half, 128 + 32);
+    }
+    // ---- the row's result
+    if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const bool seen = m != -INFINITY;
+    const int64_t out_row = (int64_t)(tile.first_token + token) * a.q_heads + qh;
+    const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + out_row;
+    const float inv = seen ? (p.splits == 1 ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 1.0f) : 0.0f;
+    uint16_t* dst = a.out.p + (int64_t)(tile.first_token + token) * a.out.token_stride +
+                    (int64_t)qh * a.out.head_stride;
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+      uint32_t v[32];
+      if (work && blocks > 0) {
+        tmem_ld32(o_addr + 32 * c, v);
+        tmem_wait_ld();
+      }
+      if (!live) continue;
+      float o[32];
+#pragma unroll
+      for (int x = 0; x < 32; ++x) o[x] = seen ? __uint_as_float(v[x]) * inv : 0.0f;
+      if (p.splits == 1) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t w[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            if (a.dtype == kDTypeBF16) {
+              const __nv_bfloat162 h = __floats2bfloat162_rn(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
+              w[y] = *reinterpret_cast<const uint32_t*>(&h);
+            } else {
+              w[y] = pack_h2(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
+            }
+          }
+          *reinterpret_cast<uint4*>(dst + 32 * c + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          *reinterpret_cast<float4*>(p.part_o + part_row * kD + 32 * c + 4 * x) =
+              make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+      }
+    }
+    if (live) {
+      if (p.splits > 1)
+        *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
+      else if (a.lse)
+        a.lse[out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
+    }
+  }
+  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+template <int kD>
+cudaError_t launch_d(const Params& p, cudaStream_t stream) {
+  constexpr int kSmem = PromptShape<kD>::kSmem;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(prompt_kernel<kD>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
+  prompt_kernel<kD><<<grid, kPThreads, kSmem, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_prompt(const Params& p, cudaStream_t stream) {
+  if (p.a.cache.head_size == 64) return launch_d<64>(p, stream);
+  if (p.a.cache.head_size == 128) return launch_d<128>(p, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace kv
+}  // namespace ssw
