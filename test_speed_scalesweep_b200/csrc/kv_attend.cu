@@ -259,20 +259,23 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[h][n][c] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < S::kKSteps; ++j) {
-        uint32_t f[2];  // the scale of this step's block, twice
+      for (int w = 0; w < kKWords; ++w) {
+        // a word holds two steps of the same block; its scale, twice
+        uint32_t x[2][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t two = e4m3_h2(sc[r] >> (16 * (j / 8)));
-          f[r] = __byte_perm(two, two, (j / 4) & 1 ? 0x3232 : 0x1010);
-        }
-        const int word = j / 2, byte = 2 * (j & 1);
-        const uint32_t a0 = mul_h2(e2m1_h2(kw[0][word], byte), f[0]);
-        const uint32_t a1 = mul_h2(e2m1_h2(kw[1][word], byte), f[1]);
-        const uint32_t a2 = mul_h2(e2m1_h2(kw[0][word], byte + 1), f[0]);
-        const uint32_t a3 = mul_h2(e2m1_h2(kw[1][word], byte + 1), f[1]);
+          const uint32_t two = e4m3_h2(sc[r] >> (16 * (w / 4)));
+          const uint32_t f = __byte_perm(two, two, (w / 2) & 1 ? 0x3232 : 0x1010);
+          e2m1_h2x4(kw[r][w], x[r]);
 #pragma unroll
-        for (int n = 0; n < kNT; ++n) mma16816(s[h][n], a0, a1, a2, a3, q[n][j][0], q[n][j][1]);
+          for (int b = 0; b < 4; ++b) x[r][b] = mul_h2(x[r][b], f);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < kNT; ++n)
+            mma16816(s[h][n], x[0][2 * u], x[1][2 * u], x[0][2 * u + 1], x[1][2 * u + 1],
+                     q[n][2 * w + u][0], q[n][2 * w + u][1]);
       }
     }
 
@@ -371,18 +374,25 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           even[u] = (x & 0x0F0F0F0Fu) | ((y << 4) & 0xF0F0F0F0u);
           odd[u] = ((x >> 4) & 0x0F0F0F0Fu) | (y & 0xF0F0F0F0u);
         }
+        const int fi = kD == 256 ? w / 2 : 0;
+        uint32_t he[2][4], ho[2][4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          // tile w * 4 + b: row g is d = g * D/8 + 8 w + 2 b, row g + 8 the next
-          const int fi = kD == 256 ? w / 2 : 0;
-          const uint32_t a0 = mul_h2(e2m1_h2(even[0], b), f[0][fi]);
-          const uint32_t a1 = mul_h2(e2m1_h2(odd[0], b), f[0][fi]);
-          const uint32_t a2 = mul_h2(e2m1_h2(even[1], b), f[1][fi]);
-          const uint32_t a3 = mul_h2(e2m1_h2(odd[1], b), f[1][fi]);
+        for (int u = 0; u < 2; ++u) {
+          e2m1_h2x4(even[u], he[u]);
+          e2m1_h2x4(odd[u], ho[u]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            he[u][b] = mul_h2(he[u][b], f[u][fi]);
+            ho[u][b] = mul_h2(ho[u][b], f[u][fi]);
+          }
+        }
+        // tile w * 4 + b: row g is d = g * D/8 + 8 w + 2 b, row g + 8 the next
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
           for (int n = 0; n < kNT; ++n)
-            mma16816(acc[n][w * 4 + b], a0, a1, a2, a3, pt[h][n][0], pt[h][n][1]);
-        }
+            mma16816(acc[n][w * 4 + b], he[0][b], ho[0][b], he[1][b], ho[1][b], pt[h][n][0],
+                     pt[h][n][1]);
       }
     }
     __syncwarp();  // every lane has read the stage before it is filled again

@@ -183,9 +183,10 @@ __device__ __forceinline__ void store_row(const RowRegs<kD>& r, uint32_t tile, i
     const uint32_t f = __byte_perm(two, two, b & 1 ? 0x3232 : 0x1010);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t w = r.codes[2 * b + h];
-      st_shared16(tile + tile_offset(row, 2 * b + h), mul_h2(e2m1_h2(w, 0), f),
-                  mul_h2(e2m1_h2(w, 1), f), mul_h2(e2m1_h2(w, 2), f), mul_h2(e2m1_h2(w, 3), f));
+      uint32_t x[4];
+      e2m1_h2x4(r.codes[2 * b + h], x);
+      st_shared16(tile + tile_offset(row, 2 * b + h), mul_h2(x[0], f), mul_h2(x[1], f),
+                  mul_h2(x[2], f), mul_h2(x[3], f));
     }
   }
 }
