@@ -26,6 +26,7 @@
 // (relative 2^-11, finer than a bf16 result) scaled by 2^kShift, so that
 // weights down to 2^-(14 + kShift) of the largest keep full precision.
 #include <cstdint>
+#include <cstdlib>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -46,7 +47,7 @@ struct Shape {
   static constexpr int kCodeRow = kD / 2, kScaleRow = kD / 16;
   static constexpr int kKCodes = kKeys * kCodeRow, kKScales = kKeys * kScaleRow;
   static constexpr int kStage = 2 * (kKCodes + kKScales);
-  static constexpr int kStages = kD == 256 ? 2 : 4;
+  static constexpr int kStages = kD == 256 ? 2 : 3;
   static constexpr int kRing = kStages * kStage;           // of a warp
   static constexpr int kKSteps = kD / 16;
 };
@@ -60,14 +61,20 @@ constexpr int smem_bytes() {
   return (ring > merge ? ring : merge) + kWarps * Shape<kD>::kStages * 8;
 }
 
+template <bool kOn>
+struct Flag {
+  static constexpr bool value = kOn;
+};
+
 template <int kD, int kNT>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1) decode_kernel(const Params p) {
   using S = Shape<kD>;
   constexpr int kRows = kNT * 8;
   constexpr int kQuarter = kD / 4;             // elements of a key row per thread
   constexpr int kKWords = kD / 32;             // 32-bit words of codes per thread and key row
   constexpr int kVWords = kD / 64 < 1 ? 1 : kD / 64;  // words of codes per thread and value row
   extern __shared__ __align__(128) uint8_t smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.y, head = blockIdx.z;
@@ -100,42 +107,46 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   const int64_t side_scale = (int64_t)a.cache.kv_heads * page_rows * S::kScaleRow;
   // lane l < 4 * pieces copies part l & 3 (K codes, K scales, V codes, V scales) of piece l >> 2
   const int part = lane & 3, my_piece = lane >> 2;
+  const bool copies = my_piece < pieces;
+  const bool scales_part = part & 1, value_part = part & 2;
+  const int row_bytes = scales_part ? S::kScaleRow : S::kCodeRow;
+  const uint32_t copy_bytes = piece * row_bytes;
+  const int64_t page_stride = scales_part ? a.cache.scales_page_stride : a.cache.codes_page_stride;
+  const uint8_t* copy_src =
+      (scales_part ? a.cache.scales + (value_part ? side_scale : 0)
+                   : a.cache.codes + (value_part ? side_code : 0)) +
+      (int64_t)head * page_rows * row_bytes;
+  const uint32_t copy_dst = ring + (value_part ? S::kKCodes + S::kKScales : 0) +
+                            (scales_part ? S::kKCodes : 0) + my_piece * copy_bytes;
+  const int copy_key = c0 + warp * kKeys + my_piece * piece;  // of stage 0
+  const int copy_end = copies ? min((int64_t)tile.end, (int64_t)c0 + p.chunk) : 0;
   auto page_of = [&](int i) -> int {  // the page of this lane's piece of stage i, or -1
-    const int k = c0 + (warp + i * kWarps) * kKeys + my_piece * piece;
-    if (my_piece >= pieces || i >= n_stages || k >= tile.end) return -1;
+    const int k = copy_key + i * (kWarps * kKeys);
+    if (k >= copy_end) return -1;
     const int pg = __ldg(table + (k >> p.page_shift));
     return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
   };
-  auto issue = [&](int i, int pg) {
-    const uint32_t bar = bars + 8 * (i % S::kStages);
-    const uint32_t live = __ballot_sync(0xFFFFFFFFu, pg >= 0 && my_piece < pieces);
+  // Starts stage i's copies into ring slot `slot`; which lanes' pieces exist.
+  auto issue = [&](int i, int slot, int pg) -> uint32_t {
+    const uint32_t bar = bars + 8 * slot;
+    const uint32_t live = __ballot_sync(0xFFFFFFFFu, pg >= 0);
     if (lane == 0)
       mbar_expect_tx(bar, (uint32_t)(__popc(live) / 4) * (uint32_t)(S::kStage / kKeys * piece));
     __syncwarp();
-    if (pg >= 0 && my_piece < pieces) {
-      const int k = c0 + (warp + i * kWarps) * kKeys + my_piece * piece;
-      const int64_t row = (int64_t)head * page_rows + (k & (page_rows - 1));
-      const bool scales = part & 1, value = part & 2;
-      const uint32_t bytes = piece * (scales ? S::kScaleRow : S::kCodeRow);
-      const uint8_t* src =
-          scales ? a.cache.scales + pg * a.cache.scales_page_stride + (value ? side_scale : 0) +
-                       row * S::kScaleRow
-                 : a.cache.codes + pg * a.cache.codes_page_stride + (value ? side_code : 0) +
-                       row * S::kCodeRow;
-      const uint32_t dst = ring + (i % S::kStages) * S::kStage +
-                           (value ? S::kKCodes + S::kKScales : 0) + (scales ? S::kKCodes : 0) +
-                           my_piece * bytes;
-      bulk_load(dst, src, bytes, bar);
+    if (pg >= 0) {
+      const int k = copy_key + i * (kWarps * kKeys);
+      bulk_load(copy_dst + slot * S::kStage,
+                copy_src + pg * page_stride + (k & (page_rows - 1)) * row_bytes, copy_bytes, bar);
     }
     return live;
   };
   // Which pieces of a stage in flight came, two bits a stage (bit 0: piece 0).
   uint32_t present = 0;
-  auto note = [&](int i, uint32_t live) {
-    const int at = 2 * (i % S::kStages);
+  auto note = [&](int slot, uint32_t live) {
+    const int at = 2 * slot;
     present = (present & ~(3u << at)) | (((live & 1u) | ((live >> 3) & 2u)) << at);
   };
-  for (int i = 0; i < S::kStages && i < n_stages; ++i) note(i, issue(i, page_of(i)));
+  for (int i = 0; i < S::kStages && i < n_stages; ++i) note(i, issue(i, i, page_of(i)));
   int next_page = page_of(S::kStages);
 
   // ---- queries: B fragments of f16, permuted as the keys are
@@ -143,7 +154,10 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   float scale[kNT][2];
   int lo_key[kNT][2], hi_key[kNT][2];
   float acc[kNT][kD / 16][4], m[kNT][2], l[kNT][2];
-  const float to_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  // the sign of the scale goes into Q, so that a larger score is a larger weight
+  const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  const float to_log2 = fabsf(signed_log2);
+  const bool flip = signed_log2 < 0.0f;
 #pragma unroll
   for (int n = 0; n < kNT; ++n) {
     const int r = n * 8 + g;
@@ -175,12 +189,16 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       // exponents 1..253: 2^(127 - e) is a normal number; zero, subnormal, the
       // largest and non-finite rows are left as they are
       const bool sized = e >= 1 && e <= 253;
-      const float down = sized ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+      const float size = sized ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+      const float down = flip ? -size : size;
       row_scale = sized ? to_log2 * __uint_as_float((uint32_t)e << 23) : to_log2;
 #pragma unroll
       for (int j = 0; j < kQuarter / 2; ++j)
         w[j] = pack_h2(__uint_as_float(w[j] << 16) * down,
                        __uint_as_float(w[j] & 0xFFFF0000u) * down);
+    } else if (flip) {
+#pragma unroll
+      for (int j = 0; j < kQuarter / 2; ++j) w[j] ^= 0x80008000u;
     }
 #pragma unroll
     for (int j = 0; j < S::kKSteps; ++j) {
@@ -190,7 +208,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
     // columns 2t, 2t + 1 of the score tile are rows n * 8 + 2t, + 1
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      scale[n][c] = __shfl_sync(0xFFFFFFFFu, row_scale, (2 * t + c) * 4);
+      // never zero, or a masked score would be NaN
+      scale[n][c] = fmaxf(__shfl_sync(0xFFFFFFFFu, row_scale, (2 * t + c) * 4), 1e-37f);
       const int rr = n * 8 + 2 * t + c;
       const int pos = tile.offset + (tile.row0 + rr) / p.group;
       const bool there = rr < tile.rows;
@@ -211,12 +230,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   // thread pairs lie in rows t, t + 4, t + 8, t + 12.
   const int key_a = (g >> 1) + (g & 1) * 4;  // pi(g); pi(g + 8) = pi(g) + 8
   bool ok = true;
+  int slot = 0;
+  uint32_t phase = 0;
   for (int i = 0; i < n_stages; ++i) {
-    const int slot = i % S::kStages;
     const int k0 = c0 + (warp + i * kWarps) * kKeys;
     const int page_ahead = next_page;
     next_page = page_of(i + 1 + S::kStages);
-    if (!mbar_wait(bars + 8 * slot, (i / S::kStages) & 1)) {
+    if (!mbar_wait(bars + 8 * slot, phase)) {
       // give up: the copies still in flight get their (bounded) time to land
       for (int j = i; j < n_stages && j < i + S::kStages; ++j)
         mbar_wait(bars + 8 * (j % S::kStages), (j / S::kStages) & 1);
@@ -232,6 +252,9 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
     const bool masked = k0 < tile.all_beg || k0 + kKeys > tile.all_end || k0 + kKeys > c1 ||
                         came != (pieces == 2 ? 3u : 1u);
 
+    // One stage; without masks where every row of the tile sees all its keys.
+    auto attend = [&](auto mask_tag) {
+    constexpr bool masked = decltype(mask_tag)::value;
     // S^T = K Q^T
     float s[2][kNT][4];
 #pragma unroll
@@ -258,6 +281,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       for (int n = 0; n < kNT; ++n)
 #pragma unroll
         for (int c = 0; c < 4; ++c) s[h][n][c] = 0.0f;
+      // two chains of accumulation, for the products' latency
+      float s2[kNT][4] = {};
 #pragma unroll
       for (int w = 0; w < kKWords; ++w) {
         // a word holds two steps of the same block; its scale, twice
@@ -274,9 +299,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int n = 0; n < kNT; ++n)
-            mma16816(s[h][n], x[0][2 * u], x[1][2 * u], x[0][2 * u + 1], x[1][2 * u + 1],
-                     q[n][2 * w + u][0], q[n][2 * w + u][1]);
+            mma16816(u ? s2[n] : s[h][n], x[0][2 * u], x[1][2 * u], x[0][2 * u + 1],
+                     x[1][2 * u + 1], q[n][2 * w + u][0], q[n][2 * w + u][1]);
       }
+#pragma unroll
+      for (int n = 0; n < kNT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[h][n][c] += s2[n][c];
     }
 
     // softmax over this stage's keys, in units of log2
@@ -289,8 +318,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float v = s[h][n][c] * scale[n][c & 1];
-          if (masked) {
+          float v = s[h][n][c];
+          if constexpr (masked) {
             const int key = k0 + h * 16 + key_a + 8 * (c >> 1);
             const bool here = (came >> (pieces == 2 ? h : 0)) & 1u;
             if (!here || key >= c1 || key > hi_key[n][c & 1] || key < lo_key[n][c & 1])
@@ -304,6 +333,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
         mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 4));
         mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 8));
         mx[c] = fmaxf(mx[c], __shfl_xor_sync(0xFFFFFFFFu, mx[c], 16));
+        mx[c] *= scale[n][c];
         grow |= mx[c] > m[n][c] + kSlack;
       }
       if (__any_sync(0xFFFFFFFFu, grow)) {
@@ -324,8 +354,10 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
       const float m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - kShift;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float p0 = ex2(s[h][n][0] - m0), p1 = ex2(s[h][n][1] - m1);
-        const float p2 = ex2(s[h][n][2] - m0), p3 = ex2(s[h][n][3] - m1);
+        const float p0 = ex2(fmaf(s[h][n][0], scale[n][0], -m0));
+        const float p1 = ex2(fmaf(s[h][n][1], scale[n][1], -m1));
+        const float p2 = ex2(fmaf(s[h][n][2], scale[n][0], -m0));
+        const float p3 = ex2(fmaf(s[h][n][3], scale[n][1], -m1));
         l[n][0] += p0 + p2;
         l[n][1] += p1 + p3;
         pt[h][n][0] = transpose8(pack_h2(p0, p1));
@@ -352,7 +384,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
           sc[r] = *reinterpret_cast<const uint16_t*>(vs + row * S::kScaleRow + 2 * g);
         }
         // what lies behind the last key may hold anything, NaN scales too
-        if (masked) {
+        if constexpr (masked) {
           const int key = k0 + row;
           const bool here = (came >> (pieces == 2 ? h : 0)) & 1u;
           if (!here || key >= c1 || key < tile.beg) sc[r] = 0;
@@ -395,8 +427,17 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
                      pt[h][n][1]);
       }
     }
+    };
+    if (masked)
+      attend(Flag<true>());
+    else
+      attend(Flag<false>());
     __syncwarp();  // every lane has read the stage before it is filled again
-    if (i + S::kStages < n_stages) note(i + S::kStages, issue(i + S::kStages, page_ahead));
+    if (i + S::kStages < n_stages) note(slot, issue(i + S::kStages, slot, page_ahead));
+    if (++slot == S::kStages) {
+      slot = 0;
+      phase ^= 1;
+    }
   }
   if (!ok && lane == 0 && a.status) atomicCAS(a.status, 0, 1);
 
@@ -464,50 +505,78 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const Params p) {
   }
 }
 
-// Joins the splits of a tile's rows in their order: one warp per row.
+// Joins the splits of one row, always in the same order: warp w takes splits w,
+// w + 4, ..., then the warps' results are joined.  A programmatic dependent of
+// the kernel that wrote them.
 template <int kD>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile_rows) {
+  constexpr int kPer = kD / 32;  // elements of a lane
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.z, seq = blockIdx.x / p.tiles;
+  const int head = blockIdx.z, seq = blockIdx.x / p.tiles, r = blockIdx.y;
+  __shared__ float part[kWarps][kD];
+  __shared__ float part_m[kWarps], part_l[kWarps];
   Tile tile;
-  if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile)) return;
+  if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) return;
   const int splits = used_splits(p, tile);
+  const int row = tile.row0 + r, token = tile.first_token + row / p.group;
+  const int qh = head * p.group + row % p.group;
+  const int64_t out_row = (int64_t)token * a.q_heads + qh;
+  const int64_t step = a.tokens * a.q_heads;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
+  const float* po = p.part_o + out_row * kD + lane * kPer;
   const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
-  for (int r = blockIdx.y * kWarps + warp; r < tile.rows; r += gridDim.y * kWarps) {
-    const int row = tile.row0 + r, token = tile.first_token + row / p.group;
-    const int qh = head * p.group + row % p.group;
-    const int64_t out_row = (int64_t)token * a.q_heads + qh;
-    const int64_t step = a.tokens * a.q_heads;
-    float mm = -INFINITY;
-    for (int s = lane; s < splits; s += 32) mm = fmaxf(mm, p.part_ml[(s * step + out_row) * 2]);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float mm = -INFINITY;
+  for (int s = warp + lane * kWarps; s < splits; s += 32 * kWarps) mm = fmaxf(mm, ml[s * step].x);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
-    float sum = 0.0f, acc[kD / 32];
+  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
+  float sum = 0.0f, acc[kPer];
 #pragma unroll
-    for (int j = 0; j < kD / 32; ++j) acc[j] = 0.0f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (s * step + out_row) * 2);
-      const float f = mm == -INFINITY ? 0.0f : ex2(ml.x - mm);
-      sum += f * ml.y;
-      const float* o = p.part_o + (s * step + out_row) * kD;
+  for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
+#pragma unroll 4
+  for (int s = warp; s < splits; s += kWarps) {
+    const float2 x = ml[s * step];
+    float v[kPer];
 #pragma unroll
-      for (int j = 0; j < kD / 64; ++j) {
-        const float2 v = *reinterpret_cast<const float2*>(o + j * 64 + lane * 2);
-        acc[2 * j] += f * v.x;
-        acc[2 * j + 1] += f * v.y;
-      }
-    }
-    const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;
-    uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
+    for (int j = 0; j < kPer / 2; ++j)
+      *reinterpret_cast<float2*>(v + 2 * j) = *reinterpret_cast<const float2*>(po + s * step * kD + 2 * j);
+    const float f = mm == -INFINITY ? 0.0f : ex2(x.x - mm);
+    sum += f * x.y;
 #pragma unroll
-    for (int j = 0; j < kD / 64; ++j) {
-      const float v[2] = {acc[2 * j] * inv, acc[2 * j + 1] * inv};
-      store16(dst + j * 64 + lane * 2, v, a.dtype);
-    }
-    if (lane == 0 && a.lse)
-      a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+    for (int j = 0; j < kPer; ++j) acc[j] += f * v[j];
   }
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = acc[j];
+  if (lane == 0) {
+    part_m[warp] = mm;
+    part_l[warp] = sum;
+  }
+  __syncthreads();
+  float all = part_m[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) all = fmaxf(all, part_m[w]);
+  float f[kWarps], total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    f[w] = all == -INFINITY ? 0.0f : ex2(part_m[w] - all);
+    total += f[w] * part_l[w];
+  }
+  const float inv = all == -INFINITY ? 0.0f : inv_mult / total;
+  uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
+  for (int d = threadIdx.x * 2; d < kD; d += kThreads * 2) {
+    float v[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      v[0] += f[w] * part[w][d];
+      v[1] += f[w] * part[w][d + 1];
+    }
+    v[0] *= inv;
+    v[1] *= inv;
+    store16(dst + d, v, a.dtype);
+  }
+  if (threadIdx.x == 0 && a.lse)
+    a.lse[out_row] = all == -INFINITY ? -INFINITY : (all - kShift + log2f(total)) * kLn2;
 }
 
 int log2i(int v) {
@@ -528,6 +597,8 @@ struct Plan {
 
 // `most` rows at most per sequence; `target` CTAs keep the GPU busy evenly.
 Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int64_t min_chunk) {
+  if (tile_rows < 256 && getenv("SSW_T")) target = atoi(getenv("SSW_T")) * 148;
+  if (tile_rows < 256 && getenv("SSW_C")) min_chunk = atoi(getenv("SSW_C"));
   Cut c;
   c.rows = tile_rows;
   c.tiles = (int)((most + tile_rows - 1) / tile_rows);
@@ -597,6 +668,22 @@ cudaError_t launch_rows(const Params& p, int rows, cudaStream_t stream) {
   return cudaErrorInvalidValue;
 }
 
+template <int kD>
+cudaError_t launch_join(const Params& p, int tile_rows, cudaStream_t stream) {
+  const int64_t most = (int64_t)p.a.max_query_len * p.group;  // rows of a sequence
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), (unsigned)(most < tile_rows ? most : tile_rows),
+                     p.a.cache.kv_heads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<kD>, p, tile_rows);
+}
+
 cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
   if (c.rows == 0) return cudaSuccess;
   p.tiles = c.tiles;
@@ -610,12 +697,9 @@ cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
                   : d == 128            ? launch_rows<128>(p, c.rows, stream)
                                         : launch_rows<256>(p, c.rows, stream);
   if (e != cudaSuccess || c.splits == 1) return e;
-  const dim3 grid((unsigned)(p.a.seqs * p.tiles), (c.rows + kWarps - 1) / kWarps,
-                  p.a.cache.kv_heads);
-  if (d == 64) join_kernel<64><<<grid, kThreads, 0, stream>>>(p, c.rows);
-  else if (d == 128) join_kernel<128><<<grid, kThreads, 0, stream>>>(p, c.rows);
-  else join_kernel<256><<<grid, kThreads, 0, stream>>>(p, c.rows);
-  return cudaGetLastError();
+  return d == 64    ? launch_join<64>(p, c.rows, stream)
+         : d == 128 ? launch_join<128>(p, c.rows, stream)
+                    : launch_join<256>(p, c.rows, stream);
 }
 
 }  // namespace

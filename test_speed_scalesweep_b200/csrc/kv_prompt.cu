@@ -195,6 +195,7 @@ template <int kD>
 __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   using S = PromptShape<kD>;
   extern __shared__ uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
@@ -352,6 +353,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
         scale *= __uint_as_float((uint32_t)e << 23);
       }
     }
+    scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
     if (flip) down = -down;
 #pragma unroll 4
     for (int j = 0; j < kD / 8; ++j) {
