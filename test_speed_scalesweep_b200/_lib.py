@@ -164,19 +164,18 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class _Nothing:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+_kv = None
 
 
-_NOTHING = _Nothing()
-
-
-def on_device(device: torch.device):
-    """``torch.cuda.device(device)``, at no cost where it is the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NOTHING
-    return torch.cuda.device(device)
+def kv_binding():
+    """The native binding of the KV-cache operators (``_kv_binding.so``)."""
+    global _kv
+    if _kv is None:
+        lib()  # the library it links to: the same checks, the same error
+        if not os.path.exists(_build.BINDING_PATH):
+            raise RuntimeError(
+                f"{_build.BINDING_PATH} is missing: it is built with the CUDA library "
+                "(python -m test_speed_scalesweep_b200.build); there is no fallback")
+        from . import _kv_binding
+        _kv = _kv_binding
+    return _kv

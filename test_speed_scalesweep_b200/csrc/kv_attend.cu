@@ -26,7 +26,6 @@
 // (relative 2^-11, finer than a bf16 result) scaled by 2^kShift, so that
 // weights down to 2^-(14 + kShift) of the largest keep full precision.
 #include <cstdint>
-#include <cstdlib>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -597,8 +596,6 @@ struct Plan {
 
 // `most` rows at most per sequence; `target` CTAs keep the GPU busy evenly.
 Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int64_t min_chunk) {
-  if (tile_rows < 256 && getenv("SSW_T")) target = atoi(getenv("SSW_T")) * 148;
-  if (tile_rows < 256 && getenv("SSW_C")) min_chunk = atoi(getenv("SSW_C"));
   Cut c;
   c.rows = tile_rows;
   c.tiles = (int)((most + tile_rows - 1) / tile_rows);
@@ -621,16 +618,22 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t rows = (int64_t)a.max_query_len * group;
   const int most = a.cache.head_size == 256 ? 16 : 32;  // rows of decode_kernel's largest tile
+  // A single sequence is cut into one wave of CTAs (1 x 131072 keys, 8 kv heads:
+  // 53 us with 3 CTAs per SM, 57 with 8, 70 with 12, each with a start and a
+  // partial result of its own).  Sequences of several lengths are cut finer, so
+  // that the longest do not run on alone (64 of up to 8192: 100 us with 24,
+  // 111 with 12, 117 with 72).
+  const int64_t target = (int64_t)device_sms * (a.seqs == 1 ? 3 : 24);
   Plan pl = {};
   if (rows <= most || a.cache.head_size == 256) {
-    pl.decode = cut_of(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, (int64_t)device_sms * 12, 256);
+    pl.decode = cut_of(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, target, 128);
     pl.decode.max_rows = 0x7FFFFFFF;
     return pl;
   }
   pl.prompt = cut_of(a, kPromptRows, rows, device_sms, 512);
   pl.prompt.max_rows = 0x7FFFFFFF;
   if (a.seqs > 1) {  // single tokens among prompts
-    pl.decode = cut_of(a, group <= 8 ? 8 : 16, 16, (int64_t)device_sms * 12, 256);
+    pl.decode = cut_of(a, group <= 8 ? 8 : 16, 16, target, 128);
     pl.decode.max_rows = pl.decode.rows;
     pl.decode.tiles = 1;
     pl.prompt.min_rows = pl.decode.rows + 1;

@@ -21,7 +21,6 @@ stands for ``code * scale / multiplier``.  A token's slot is
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -96,68 +95,6 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
     return torch.cat([angle.cos() * mult, angle.sin() * mult], dim=-1).float()
 
 
-def cache_struct(codes: torch.Tensor, scales: torch.Tensor,
-                 kv_input_scale: torch.Tensor | None) -> _lib.KVCache:
-    """Check one layer's cache tensors and describe them to the C ABI."""
-    if codes.dim() != 5 or scales.dim() != 5:
-        raise ValueError("codes and scales must be [num_pages, 2, kv_heads, page_size, ..] tensors")
-    pages, two, heads, page, half = codes.shape
-    if codes.dtype != torch.uint8 or scales.dtype != torch.float8_e4m3fn:
-        raise ValueError("codes must be uint8 and scales float8_e4m3fn, got "
-                         f"{codes.dtype} and {scales.dtype}")
-    if two != 2 or scales.shape != (pages, 2, heads, page, half // 8):
-        raise ValueError("codes must be [num_pages, 2, kv_heads, page_size, head_size/2] and scales "
-                         f"[.., head_size/16], got {tuple(codes.shape)} and {tuple(scales.shape)}")
-    dev = codes.device
-    if dev.type != "cuda":
-        raise ValueError("codes must be a CUDA tensor (there is no CPU implementation)")
-    if scales.device != dev:
-        raise ValueError(f"scales must be on {dev}, got {scales.device}")
-    sc, ss = codes.stride(), scales.stride()
-    row, srow = page * half, page * (half // 8)
-    if (sc[1:] != (heads * row, row, half, 1)
-            or ss[1:] != (heads * srow, srow, half // 8, 1)):
-        raise ValueError("codes and scales must be contiguous within a page")
-    mult = 0
-    if kv_input_scale is not None:
-        if (kv_input_scale.dtype != torch.float32 or kv_input_scale.shape != (2,)
-                or kv_input_scale.device != dev or kv_input_scale.stride(0) != 1):
-            raise ValueError(f"kv_input_scale must be a contiguous float32 tensor of shape [2] on {dev}")
-        mult = kv_input_scale.data_ptr()
-    return _lib.KVCache(codes.data_ptr(), scales.data_ptr(), sc[0], ss[0], mult, pages, page, heads,
-                        half * 2)
-
-
-def heads_struct(name: str, t: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype,
-                 device: torch.device) -> _lib.KVHeads:
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}, got {t.dtype} "
-                         f"{list(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    st, sh, sd = t.stride()
-    # the stride of an axis of length 1 says nothing, and may be anything
-    if shape[0] <= 1:
-        st = 0
-    if shape[1] <= 1:
-        sh = 0
-    if sd != 1 or st % 8 or sh % 8:
-        raise ValueError(f"{name}: the last dimension must be contiguous, the other strides "
-                         "multiples of 8")
-    return _lib.KVHeads(t.data_ptr(), st, sh)
-
-
-def check_distinct(name: str, t: torch.Tensor) -> None:
-    """Refuse an output whose elements share memory (an expanded tensor)."""
-    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
-        raise ValueError(f"{name} must not be an expanded tensor")
-
-
-def _check_index(name: str, t: torch.Tensor, n: int, device: torch.device) -> None:
-    if t.dtype != torch.int64 or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int64 tensor of shape [{n}] on {device}")
-
-
 def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
                                          value: torch.Tensor, positions: torch.Tensor,
                                          cos_sin_cache: torch.Tensor, slot_mapping: torch.Tensor,
@@ -179,39 +116,8 @@ def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
     read.  Rows whose slot is negative or past the last page are padding: not
     stored.  Slots must be distinct.  A position outside the table gives NaN in
     the query, and that token is not stored."""
-    cache = cache_struct(codes, scales, kv_input_scale)
-    if kv_input_scale is None:
-        raise ValueError("kv_input_scale is required")
-    dev = codes.device
-    if query.dim() != 3:
-        raise ValueError(f"query must be [T, heads, head_size], got shape {tuple(query.shape)}")
-    tokens, hq, d = query.shape
-    if d != cache.head_size:
-        raise ValueError(f"query has head size {d}, the cache {cache.head_size}")
-    dtype = _lib.dtype_code(query)
-    kv_shape = (tokens, cache.kv_heads, d)
-    q = heads_struct("query", query, (tokens, hq, d), query.dtype, dev)
-    k = heads_struct("key", key, kv_shape, query.dtype, dev)
-    v = heads_struct("value", value, kv_shape, query.dtype, dev)
-    _check_index("positions", positions, tokens, dev)
-    _check_index("slot_mapping", slot_mapping, tokens, dev)
-    if (cos_sin_cache.dtype != torch.float32 or cos_sin_cache.dim() != 2
-            or cos_sin_cache.device != dev or not cos_sin_cache.is_contiguous()):
-        raise ValueError("cos_sin_cache must be a contiguous float32 tensor [max_position, "
-                         f"rotary_dim] on {dev}")
-    if query_out is None:
-        query_out = torch.empty((tokens, hq, d), dtype=query.dtype, device=dev)
-    o = heads_struct("query_out", query_out, (tokens, hq, d), query.dtype, dev)
-    check_distinct("query_out", query_out)
-    max_position, rotary_dim = cos_sin_cache.shape
-    with _lib.on_device(dev):
-        st = _lib.lib().ssw_rotary_scalesweep_mse_nvfp4_kv_write(
-            ctypes.byref(cache), dtype, tokens, hq, ctypes.byref(q), ctypes.byref(k),
-            ctypes.byref(v), ctypes.byref(o), positions.data_ptr(), cos_sin_cache.data_ptr(),
-            max_position, rotary_dim, bool(is_neox), slot_mapping.data_ptr(),
-            _lib.stream_handle(dev))
-    _lib.check(st)
-    return query_out
+    return _lib.kv_binding().write(query, key, value, positions, cos_sin_cache, slot_mapping,
+                                   kv_input_scale, codes, scales, is_neox, query_out)
 
 
 def nvfp4_kv_gather(codes: torch.Tensor, scales: torch.Tensor, kv_input_scale: torch.Tensor,
@@ -220,20 +126,4 @@ def nvfp4_kv_gather(codes: torch.Tensor, scales: torch.Tensor, kv_input_scale: t
     (key, value), each [T, kv_heads, head_size] and contiguous.  Zeros for a
     slot outside the cache.  For a cache's readers that want plain keys and
     values: another engine's cache, or a check of what the quantizer kept."""
-    cache = cache_struct(codes, scales, kv_input_scale)
-    if kv_input_scale is None:
-        raise ValueError("kv_input_scale is required")
-    dev = codes.device
-    if dtype not in _lib.DTYPE_CODES:
-        raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
-    _check_index("slot_mapping", slot_mapping, slot_mapping.numel(), dev)
-    n = slot_mapping.numel()
-    shape = (n, cache.kv_heads, cache.head_size)
-    key = torch.empty(shape, dtype=dtype, device=dev)
-    value = torch.empty(shape, dtype=dtype, device=dev)
-    with _lib.on_device(dev):
-        st = _lib.lib().ssw_nvfp4_kv_gather(ctypes.byref(cache), _lib.DTYPE_CODES[dtype], n,
-                                            slot_mapping.data_ptr(), key.data_ptr(),
-                                            value.data_ptr(), _lib.stream_handle(dev))
-    _lib.check(st)
-    return key, value
+    return _lib.kv_binding().gather(codes, scales, kv_input_scale, slot_mapping, dtype)

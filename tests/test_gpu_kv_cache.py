@@ -168,3 +168,48 @@ def test_layer_of_a_cache_other_stream_and_graph(kv):
     want = kv.rotary_scalesweep_mse_nvfp4_kv_write(*args, *one)
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(codes[2], one[0])
+
+
+def test_refusals_of_tensors(kv):
+    """Everything that Python can pass wrongly is an error before a kernel runs."""
+    from test_speed_scalesweep_b200 import kv_attention
+    codes, scales = kv.alloc_kv_cache(4, 16, 2, 64)
+    mult, table = torch.ones(2, device="cuda"), kv.rotary_cos_sin_cache(8, 64)
+    x = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    idx = torch.zeros(3, dtype=torch.int64, device="cuda")
+
+    def write(query=x, key=x, value=x, positions=idx, cos_sin=table, slots=idx, scale=mult, c=codes, s=scales, **kw):
+        return kv.rotary_scalesweep_mse_nvfp4_kv_write(query, key, value, positions, cos_sin, slots, scale, c, s, **kw)
+
+    wide = torch.zeros(3, 2, 68, device="cuda", dtype=torch.bfloat16)[..., :64]
+    for match, kw in (
+            ("shape", dict(key=x[:2])), ("shape", dict(value=x[:, :1])), ("shape", dict(key=x.half())),
+            ("head size", dict(query=x[..., :32])), ("T, heads", dict(query=x[0])), ("bfloat16", dict(query=x.float())),
+            ("multiples of 8", dict(key=wide)), ("contiguous", dict(value=x.transpose(1, 2).contiguous().transpose(1, 2))),
+            ("on cuda", dict(key=x.cpu())), ("int64", dict(positions=idx.int())), ("int64", dict(slots=idx[:2])),
+            ("int64", dict(slots=idx.cpu())), ("cos_sin_cache", dict(cos_sin=table.double())),
+            ("cos_sin_cache", dict(cos_sin=table.t())), ("rotary_dim", dict(cos_sin=table[:, :24].contiguous())),
+            ("kv_input_scale", dict(scale=mult[:1])), ("kv_input_scale", dict(scale=None)),
+            ("within a page", dict(c=torch.zeros(4, 2, 16, 2, 32, dtype=torch.uint8, device="cuda").transpose(2, 3))),
+            ("expanded", dict(query_out=x[:1].expand(3, 2, 64))), ("query_out", dict(query_out=x[:2])),
+            ("16-byte", dict(query=torch.zeros(3 * 128 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(3, 2, 64)))):
+        with pytest.raises(ValueError, match=match):
+            write(**kw)
+    tab, lens, start = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((2, 4), (2,), (3,)))
+
+    def attend(q=x, t=tab, n=lens, s=start, mq=1, ms=16, **kw):
+        return kv_attention.nvfp4_paged_attention(q, codes, scales, mult, t, n, s, mq, ms, **kw)
+
+    for match, kw in (
+            ("multiple of the cache", dict(q=x[:, :1])), ("block_table", dict(t=tab.long())), ("block_table", dict(t=tab[0])),
+            ("contiguous", dict(t=tab.t().contiguous().t())), ("seq_lens", dict(n=lens[:1])), ("query_start", dict(s=start[:2])),
+            ("query_start", dict(s=start.cpu())), ("max_query_len", dict(mq=0)), ("max_query_len", dict(ms=0)),
+            ("integer", dict(mq=1.5)), ("window", dict(window=-1)), ("finite", dict(softmax_scale=float("nan"))),
+            ("number", dict(softmax_scale="x")), ("status", dict(status=lens.long())), ("out", dict(out=x.half())),
+            ("expanded", dict(out=x[:1].expand(3, 2, 64)))):
+        with pytest.raises(ValueError, match=match):
+            attend(**kw)
+    before = codes.clone()
+    assert write(query=x[:0], key=x[:0], value=x[:0], positions=idx[:0], slots=idx[:0]).shape == (0, 2, 64)
+    assert attend(q=x[:0]).shape == (0, 2, 64)
+    assert torch.equal(codes, before)

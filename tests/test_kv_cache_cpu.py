@@ -54,33 +54,26 @@ def test_no_tokens_is_a_no_op(built_library):
     assert _lib.lib().ssw_nvfp4_kv_gather(ctypes.byref(cache()), 0, 0, None, None, None, None) == 0
 
 
-def test_python_refuses_cpu_and_wrong_tensors():
+def test_python_refuses_cpu_and_wrong_tensors(built_library):
     codes, scales = kv_cache.alloc_kv_cache(2, 16, 1, 64, device="cpu")
     assert codes.shape == (2, 2, 1, 16, 32) and scales.shape == (2, 2, 1, 16, 4)
+    mult, slots = torch.ones(2), torch.zeros(1, dtype=torch.int64)
     with pytest.raises(ValueError, match="CUDA"):
-        kv_cache.nvfp4_kv_gather(codes, scales, torch.ones(2), torch.zeros(1, dtype=torch.int64))
+        kv_cache.nvfp4_kv_gather(codes, scales, mult, slots)
     with pytest.raises(ValueError, match="head_size/16"):
-        kv_cache.cache_struct(codes, scales[..., :2], None)
+        kv_cache.nvfp4_kv_gather(codes, scales[..., :2], mult, slots)
     with pytest.raises(ValueError, match="uint8"):
-        kv_cache.cache_struct(codes.int(), scales, None)
+        kv_cache.nvfp4_kv_gather(codes.int(), scales, mult, slots)
     with pytest.raises(ValueError, match="num_pages"):
-        kv_cache.cache_struct(codes[0], scales[0], None)
+        kv_cache.nvfp4_kv_gather(codes[0], scales[0], mult, slots)
+    with pytest.raises(ValueError, match="codes must be a tensor"):
+        kv_cache.nvfp4_kv_gather(None, scales, mult, slots)
+    with pytest.raises(ValueError, match="bfloat16"):
+        kv_cache.nvfp4_kv_gather(codes, scales, mult, slots, torch.float32)
     for bad in (dict(page_size=24), dict(head_size=80), dict(num_pages=0), dict(num_layers=0)):
         with pytest.raises(ValueError):
             kv_cache.alloc_kv_cache(**{**dict(num_pages=2, page_size=16, kv_heads=1, head_size=64,
                                               device="cpu"), **bad})
-    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
-    dev = torch.device("cpu")
-    with pytest.raises(ValueError, match="shape"):
-        kv_cache.heads_struct("key", x, (4, 1, 64), torch.bfloat16, dev)
-    with pytest.raises(ValueError, match="contiguous"):
-        kv_cache.heads_struct("key", x.transpose(1, 2).contiguous().transpose(1, 2), (4, 2, 64),
-                              torch.bfloat16, dev)
-    with pytest.raises(ValueError, match="multiples of 8"):
-        kv_cache.heads_struct("key", torch.zeros(4, 2, 68, dtype=torch.bfloat16)[..., :64],
-                              (4, 2, 64), torch.bfloat16, dev)
-    with pytest.raises(ValueError, match="expanded"):
-        kv_cache.check_distinct("query_out", x[:1].expand(4, 2, 64))
 
 
 def test_rotary_table():
@@ -197,12 +190,12 @@ def test_pages_refusals(built_library, call, needle):
         _lib.check(st)
 
 
-def test_pages_python_refusals():
+def test_pages_python_refusals(built_library):
     from test_speed_scalesweep_b200 import kv_pages
     codes, scales = kv_cache.alloc_kv_cache(4, 16, 1, 64, device="cpu", num_layers=2)
     with pytest.raises(ValueError, match="CUDA"):
         kv_pages.NVFP4KVPages.empty(codes, scales, 2, 2)
-    with pytest.raises(ValueError, match="layers"):
+    with pytest.raises(ValueError, match="num_pages"):
         kv_pages.NVFP4KVPages.empty(codes[0, 0], scales[0, 0], 2, 2)
     with pytest.raises(ValueError, match="head_size/16"):
         kv_pages.NVFP4KVPages.empty(codes, scales[..., :2], 2, 2)
