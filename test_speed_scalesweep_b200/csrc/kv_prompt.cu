@@ -31,16 +31,29 @@
 
 #include "attend.cuh"
 #include "kv.cuh"
+#include "ptx.cuh"
 #include "quant.cuh"
 
 namespace ssw {
 namespace kv {
 namespace {
 
-constexpr int kPThreads = 13 * 32;
+constexpr int kPThreads = 16 * 32;
 constexpr int kBlock = 128;  // keys of a block
 constexpr int kWarpDequant = 8, kWarpMma = 12;
 constexpr int kMaskRing = 4;
+// Registers: the launch gives every thread 128.  The softmax threads hold a
+// whole row of S (128) and take what the others can spare:
+// 256 x 184 + 128 x 96 + 128 x 40 = 64512 of the launch's 65536.
+constexpr int kRegsSoftmax = 184, kRegsDequant = 96, kRegsMma = 40;
+template <int kRegs>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 
 // Named barriers: tile slots 1..4 full, P of half 0 / 1, Q loaded.
 constexpr int kBarSlot = 1, kBarP = 5, kBarQ = 7;
@@ -233,7 +246,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
   bool ok = true;
 
-  if (warp == kWarpMma) {
+  if (warp >= kWarpMma) {
+    fewer_registers<kRegsMma>();
+    if (warp == kWarpMma) {
     bar_sync(kBarQ, 256 + 32);
     auto qk = [&](int half, int slot) {
       if (lane == 0) {
@@ -284,7 +299,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       }
     }
     __syncwarp();
+    }
   } else if (warp >= kWarpDequant) {
+    fewer_registers<kRegsDequant>();
     const int i = threadIdx.x - kWarpDequant * 32;  // this thread's key of a block
     const int page_mask = (1 << p.page_shift) - 1;
     const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
@@ -327,6 +344,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       fetch(v, j + 1, pg, 1);
     }
   } else {
+    more_registers<kRegsSoftmax>();
     const int half = warp >> 2, r = (warp & 3) * 32 + lane, row_in = half * 128 + r;
     const bool live = row_in < tile.rows;
     const int row = tile.row0 + row_in, token = row / p.group, qh = head * p.group + row % p.group;
@@ -401,22 +419,23 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
           __any_sync(0xFFFFFFFFu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu);
       if (ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), j & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
-      // pass 1: the row's maximum
-      float mx = -INFINITY;
+      uint32_t v[128];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        tmem_ld32(s_addr + 32 * c, v);
-        tmem_wait_ld();
-        if (masked) {
+      for (int c = 0; c < 4; ++c)
+        tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+      tmem_wait_ld();
+      if (masked) {
 #pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (!((mask[c] >> x) & 1u)) v[x] = 0xFF800000u;
-        }
-#pragma unroll
-        for (int x = 0; x < 32; ++x) mx = fmaxf(mx, __uint_as_float(v[x]));
+        for (int x = 0; x < 128; ++x)
+          if (!((mask[x / 32] >> (x % 32)) & 1u)) v[x] = 0xFF800000u;
       }
-      mx *= scale;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int x = 0; x < 128; x += 8)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          top[y] = fmaxf(fmaxf(top[y], __uint_as_float(v[x + 2 * y])), __uint_as_float(v[x + 2 * y + 1]));
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
       if (__any_sync(0xFFFFFFFFu, mx > m + kSlack)) {
         const float mn = fmaxf(m, mx);
         const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
@@ -425,38 +444,35 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
         if (j > 0) {  // nothing is in O before the first block
 #pragma unroll 1
           for (int c = 0; c < kD / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld32(o_addr + 32 * c, v);
+            uint32_t o[32];
+            tmem_ld32(o_addr + 32 * c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
-            tmem_st32(o_addr + 32 * c, v);
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tmem_st32(o_addr + 32 * c, o);
           }
         }
       }
-      // pass 2: the weights
       const float ms = m == -INFINITY ? 0.0f : m - kShift;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
+      uint64_t sums[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        uint32_t v[32], w[16];
-        tmem_ld32(s_addr + 32 * c, v);
-        tmem_wait_ld();
-        if (masked) {
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (!((mask[c] >> x) & 1u)) v[x] = 0xFF800000u;
-        }
+        uint32_t w[16];
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const float p0 = ex2(fmaf(__uint_as_float(v[2 * x]), scale, -ms));
-          const float p1 = ex2(fmaf(__uint_as_float(v[2 * x + 1]), scale, -ms));
-          sum[(2 * x) & 3] += p0;
-          sum[(2 * x + 1) & 3] += p1;
+          const int at = 32 * c + 2 * x;
+          float e0, e1;
+          unpack2(fma2(pack2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), scale2, ms2), e0, e1);
+          const float p0 = ex2(e0), p1 = ex2(e1);
+          sums[x & 1] = add2(sums[x & 1], pack2(p0, p1));
           w[x] = pack_h2(p0, p1);
         }
         tmem_st16(s_addr + 16 * c, w);
       }
+      float sum[4];
+      unpack2(sums[0], sum[0], sum[1]);
+      unpack2(sums[1], sum[2], sum[3]);
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
