@@ -355,8 +355,9 @@ int ssw_rotary_scalesweep_mse_nvfp4_kv_write(const ssw_kv_cache* cache, int dtyp
 
 /*
  * The values at slot_mapping as 16-bit floats, key and value [tokens,
- * kv_heads, head_size] contiguous: code * scale / multiplier, the quotient
- * rounded to binary32 and then to the type; zeros for a slot outside the cache.
+ * kv_heads, head_size] contiguous: code * (scale / multiplier), the quotient
+ * and the product rounded to binary32, then to the type; zeros for a slot
+ * outside the cache.
  */
 int ssw_nvfp4_kv_gather(const ssw_kv_cache* cache, int dtype, int64_t tokens,
                         const int64_t* slot_mapping, void* key, void* value, void* stream);

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include "kv.cuh"
+#include "ptx.cuh"
 #include "quant.cuh"
 
 namespace ssw {
@@ -73,17 +74,6 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
-}
-// Eight f16 from a word of codes, two per byte (element 0 in the low nibble).
-__device__ __forceinline__ void e2m1_h2x4(uint32_t word, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(word));
 }
 __device__ __forceinline__ uint32_t e4m3_h2(uint32_t two) {
   uint32_t r;

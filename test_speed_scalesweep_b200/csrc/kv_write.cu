@@ -78,26 +78,34 @@ __device__ __forceinline__ void rotate_half8(uint4& own, const uint4& other, con
   }
 }
 
-// Both halves of 8 pairs at once (the query's form).
-template <int kDType>
-__device__ __forceinline__ void rotate_half8_both(uint4& x, uint4& y, const float* cs, int half) {
+// 8 pairs with the cosines and sines at hand: (x[j], y[j]) in the half layout,
+// neighbours within x, then within y, in the interleaved one.
+template <int kDType, bool kNeox>
+__device__ __forceinline__ void rotate_pairs(uint4& x, uint4& y, const float (&c)[8],
+                                             const float (&s)[8]) {
   uint32_t* a = reinterpret_cast<uint32_t*>(&x);
   uint32_t* b = reinterpret_cast<uint32_t*>(&y);
-  float c[8], s[8];
-  *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs));
-  *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(cs) + 1);
-  *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(cs + half));
-  *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(cs + half) + 1);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float a0, a1, b0, b1;
-    widen<kDType>(a[j], a0, a1);
-    widen<kDType>(b[j], b0, b1);
-    const float c0 = c[2 * j], c1 = c[2 * j + 1], s0 = s[2 * j], s1 = s[2 * j + 1];
-    a[j] = narrow<kDType>(add_rn(mul_rn(a0, c0), -mul_rn(b0, s0)),
-                          add_rn(mul_rn(a1, c1), -mul_rn(b1, s1)));
-    b[j] = narrow<kDType>(add_rn(mul_rn(b0, c0), mul_rn(a0, s0)),
-                          add_rn(mul_rn(b1, c1), mul_rn(a1, s1)));
+    if constexpr (kNeox) {
+      float a0, a1, b0, b1;
+      widen<kDType>(a[j], a0, a1);
+      widen<kDType>(b[j], b0, b1);
+      const float c0 = c[2 * j], c1 = c[2 * j + 1], s0 = s[2 * j], s1 = s[2 * j + 1];
+      a[j] = narrow<kDType>(add_rn(mul_rn(a0, c0), -mul_rn(b0, s0)),
+                            add_rn(mul_rn(a1, c1), -mul_rn(b1, s1)));
+      b[j] = narrow<kDType>(add_rn(mul_rn(b0, c0), mul_rn(a0, s0)),
+                            add_rn(mul_rn(b1, c1), mul_rn(a1, s1)));
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t* w = h ? b : a;
+        float u, v;
+        widen<kDType>(w[j], u, v);
+        w[j] = narrow<kDType>(add_rn(mul_rn(u, c[4 * h + j]), -mul_rn(v, s[4 * h + j])),
+                              add_rn(mul_rn(v, c[4 * h + j]), mul_rn(u, s[4 * h + j])));
+      }
+    }
   }
 }
 
@@ -116,6 +124,10 @@ __device__ __forceinline__ void rotate_pairs4(uint4& x, const float* cs, int hal
                           add_rn(mul_rn(b, c[j]), mul_rn(a, s[j])));
   }
 }
+
+// Query heads per thread: they share the position's cosines and sines (64
+// bytes for 32 bytes of a head), and their loads are in flight together.
+constexpr int kQHeads = 4;
 
 struct KernelArgs {
   WriteArgs a;
@@ -212,7 +224,7 @@ __device__ __forceinline__ void quantize_units(const KernelArgs& g, uint32_t cta
   }
 }
 
-// One unit: 8 pairs of the rotated part (or 16 elements behind it).
+// One unit: 8 pairs of the rotated part (or 16 elements behind it) of kQHeads heads.
 template <int kDType, bool kNeox>
 __device__ __forceinline__ void rotate_query_unit(const KernelArgs& g, uint32_t cta) {
   const WriteArgs& p = g.a;
@@ -222,7 +234,7 @@ __device__ __forceinline__ void rotate_query_unit(const KernelArgs& g, uint32_t 
   const uint32_t token = div_bpc(u, g.q_magic, g.q_shift);
   const uint32_t r = u - token * g.q_per_token;
   const int unit = (int)(r & ((1u << g.d16_shift) - 1));
-  const uint32_t head = r >> g.d16_shift;
+  const int head = (int)(r >> g.d16_shift) * kQHeads;
   const int half = p.rotary_dim >> 1;
   const bool turn = unit * 16 < p.rotary_dim;
   const int o1 = kNeox && turn ? unit * 8 : unit * 16;
@@ -232,21 +244,36 @@ __device__ __forceinline__ void rotate_query_unit(const KernelArgs& g, uint32_t 
   uint16_t* dst = p.q_out.p + (int64_t)token * p.q_out.token_stride +
                   (int64_t)head * p.q_out.head_stride;
   const int64_t pos = __ldg(p.positions + token);
+  const bool known = (uint64_t)pos < (uint64_t)p.max_position;
   // plain loads: the output may be the query itself
-  uint4 x = *reinterpret_cast<const uint4*>(src + o1), y = *reinterpret_cast<const uint4*>(src + o2);
-  if ((uint64_t)pos >= (uint64_t)p.max_position) {
-    x = y = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);  // NaN in both types
-  } else if (turn) {
-    const float* cs = p.cos_sin + pos * p.rotary_dim;
-    if constexpr (kNeox) {
-      rotate_half8_both<kDType>(x, y, cs + o1, half);
-    } else {
-      rotate_pairs4<kDType>(x, cs + o1 / 2, half);
-      rotate_pairs4<kDType>(y, cs + o1 / 2 + 4, half);
+  uint4 x[kQHeads], y[kQHeads];
+#pragma unroll
+  for (int h = 0; h < kQHeads; ++h)
+    if (head + h < p.q_heads) {
+      x[h] = *reinterpret_cast<const uint4*>(src + h * p.q.head_stride + o1);
+      y[h] = *reinterpret_cast<const uint4*>(src + h * p.q.head_stride + o2);
+    }
+  float c[8], s[8];
+  if (turn && known) {
+    // in the half layout pair i's angle is the table's i; in the interleaved
+    // one elements 2i and 2i + 1 are pair i
+    const float* cs = p.cos_sin + pos * p.rotary_dim + (kNeox ? o1 : o1 / 2);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      *reinterpret_cast<float4*>(c + 4 * j) = __ldg(reinterpret_cast<const float4*>(cs) + j);
+      *reinterpret_cast<float4*>(s + 4 * j) = __ldg(reinterpret_cast<const float4*>(cs + half) + j);
     }
   }
-  *reinterpret_cast<uint4*>(dst + o1) = x;
-  *reinterpret_cast<uint4*>(dst + o2) = y;
+#pragma unroll
+  for (int h = 0; h < kQHeads; ++h)
+    if (head + h < p.q_heads) {
+      if (!known)
+        x[h] = y[h] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);  // NaN in both types
+      else if (turn)
+        rotate_pairs<kDType, kNeox>(x[h], y[h], c, s);
+      *reinterpret_cast<uint4*>(dst + h * p.q_out.head_stride + o1) = x[h];
+      *reinterpret_cast<uint4*>(dst + h * p.q_out.head_stride + o2) = y[h];
+    }
 }
 
 template <int kDType, bool kNeox, int kLanes>
@@ -279,8 +306,9 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const KernelArgs g) 
 }
 
 // One thread reads one block (8 bytes of codes, a scale) of one token, head and
-// side and writes 16 values: RN16(RN32(code * scale / multiplier)), the
-// product exact.
+// side and writes 16 values: RN16(RN32(code * RN32(scale / multiplier))).  One
+// division per block: one per element made the kernel twice as long as its
+// bytes (32 us for 8192 tokens of 8 heads of 128).
 template <int kDType>
 __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherArgs p, uint32_t units,
                                                           uint32_t per_token, uint32_t magic,
@@ -307,18 +335,17 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherArgs p, ui
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
         : "=r"(s2)
         : "h"((uint16_t)__ldg(p.cache.scales + page * p.cache.scales_page_stride + at)));
-    const float s = __low2float(*reinterpret_cast<const __half2*>(&s2));
-    const float mult = __ldg(p.cache.multiplier + (is_value ? 1 : 0));
+    const float s = __fdiv_rn(__low2float(*reinterpret_cast<const __half2*>(&s2)),
+                              __ldg(p.cache.multiplier + (is_value ? 1 : 0)));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint16_t pair = (uint16_t)(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFF);
-      uint32_t h;
-      asm("{\n\t.reg .b8 b, z;\n\tmov.b16 {b, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}"
-          : "=r"(h)
-          : "h"(pair));
-      const __half2 h2 = *reinterpret_cast<const __half2*>(&h);
-      w[j] = narrow<kDType>(__fdiv_rn(mul_rn(__low2float(h2), s), mult),
-                            __fdiv_rn(mul_rn(__high2float(h2), s), mult));
+    for (int j = 0; j < 2; ++j) {
+      uint32_t h[4];
+      e2m1_h2x4(j ? c.y : c.x, h);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const __half2 h2 = *reinterpret_cast<const __half2*>(&h[k]);
+        w[4 * j + k] = narrow<kDType>(mul_rn(__low2float(h2), s), mul_rn(__high2float(h2), s));
+      }
     }
   }
   uint16_t* dst = (is_value ? p.value : p.key) +
@@ -351,7 +378,7 @@ cudaError_t launch_write(const WriteArgs& a, int device_sms, cudaStream_t stream
   g.d16_shift = log2i((int)d16);
   g.page_shift = log2i(a.cache.page_size);
   g.kv_per_token = 2u * (uint32_t)a.cache.kv_heads * d16;
-  g.q_per_token = (uint32_t)a.q_heads * d16;
+  g.q_per_token = (uint32_t)((a.q_heads + kQHeads - 1) / kQHeads) * d16;
   g.kv_units = (uint32_t)(a.tokens * g.kv_per_token);
   g.q_units = (uint32_t)(a.tokens * g.q_per_token);
   make_divider(g.kv_per_token, &g.kv_magic, &g.kv_shift);

@@ -98,6 +98,18 @@ __device__ __forceinline__ uint32_t e2m1x8(float x0, float x1, float x2, float x
   return r;
 }
 
+// Eight f16 from a word of codes, two per byte (element 0 in the low nibble).
+__device__ __forceinline__ void e2m1_h2x4(uint32_t word, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(word));
+}
+
 // ---- E4M3 -----------------------------------------------------------------
 // fp32 -> E4M3 code, nearest-even, saturating finite; NaN -> 0x7F.
 __device__ __forceinline__ uint32_t e4m3_code(float x) {

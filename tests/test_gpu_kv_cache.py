@@ -97,14 +97,18 @@ def check(kv, t, hq, hkv, d, rot, neox, dtype, page, seed=0, specials=False, in_
                 want_s[slot // page, side, :, slot % page] = es[i]
     assert np.array_equal(codes.cpu().numpy(), want_c)
     assert np.array_equal(scales.view(torch.uint8).cpu().numpy(), want_s)
-    # and back: code * scale / multiplier, rounded to binary32 and then to the type
+    # and back: code * (scale / multiplier), both rounded to binary32, then to the type
     gk, gv = kv.nvfp4_kv_gather(codes, scales, mult, slots.cuda(), DT[dtype])
     for side, g in ((0, gk), (1, gv)):
         live = (slots >= 0) & (slots < pages * page)
         at = slots[live]
         c = want_c[at // page, side, :, at % page].reshape(-1, d // 2)
         s = want_s[at // page, side, :, at % page].reshape(-1, d // 16)
-        val = oracle.dequantize(c, s, c.shape[0], d, swizzled=False) / np.float32(MULT[side])
+        one = np.full_like(s, 0x38)  # an E4M3 scale of 1
+        code = oracle.dequantize(c, one, c.shape[0], d, swizzled=False)
+        factor = (torch.from_numpy(s).view(torch.float8_e4m3fn).float().numpy() / np.float32(MULT[side]))
+        val = code * factor.repeat(16, axis=1)
+        assert val.dtype == np.float32
         full = torch.zeros(t, hkv, d, dtype=DT[dtype])
         full[live] = torch.from_numpy(val).reshape(-1, hkv, d).to(DT[dtype])
         assert torch.equal(g.cpu().float(), full.float())
