@@ -24,6 +24,15 @@ constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kChunk = kCopyThreads * 2 * 16;  // bytes that a CTA moves per item
 
+// The wide kernel of a call is a programmatic dependent of its plan: it is set
+// up while the plan runs and waits for the plan's writes.
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_plan() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Exclusive scan over the CTA (1024 threads); *total gets the sum.
 __device__ __forceinline__ int block_scan(int v, int* total) {
   __shared__ int sums[32];
@@ -106,6 +115,7 @@ __device__ __host__ __forceinline__ PagesWork work_of(int32_t* w, int64_t n, int
 
 // ---- fork: the full pages are shared, a part-filled last page is copied
 __global__ void __launch_bounds__(kPlanThreads) fork_plan(const PagesArgs a, int32_t* ws) {
+  launch_dependents();
   const PagesWork w = work_of(ws, a.n, a.n);
   const int page_mask = (1 << a.page_shift) - 1;
   int bad = 0, need = 0;
@@ -209,6 +219,7 @@ __device__ __forceinline__ void copy_pairs(const PoolArgs& c, const int32_t* sou
 __global__ void __launch_bounds__(kCopyThreads) fork_apply(const PagesArgs a, const PoolArgs c,
                                                            int32_t* ws) {
   const PagesWork w = work_of(ws, a.n, a.n);
+  wait_for_plan();
   if (w.head[1] == 0) return;
   const int i = blockIdx.x;
   if (i >= a.n) {
@@ -252,9 +263,22 @@ __global__ void __launch_bounds__(kCopyThreads) free_kernel(const PagesArgs a) {
   }
 }
 
+// The last of n ascending starts that is at most k (the first is 0): the range
+// that k lies in, empty ranges skipped.
+__device__ __forceinline__ int last_at_most(const int32_t* starts, int n, int k) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (starts[mid] <= k) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
 // ---- extend: pages for new tokens, and their slots
 __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, int64_t total_tokens,
                                                             int64_t most_pages, int32_t* ws) {
+  launch_dependents();
   const PagesWork w = work_of(ws, a.n, most_pages);
   const int page_mask = (1 << a.page_shift) - 1;
   int bad = 0, longer = 0;
@@ -314,14 +338,13 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, i
       if (len >= 0) a.seq_lens[a.seqs[i]] = len;
       continue;
     }
-    const int s = a.seqs[i], have = (int)(((int64_t)len + page_mask) >> a.page_shift);
-    const int at = w.source[i];
-    const int end = i + 1 < a.n ? w.source[i + 1] : need;
-    for (int j = at; j < end; ++j) {
-      a.block_table[s * a.table_stride + have + (j - at)] = w.fresh[j];
-      a.refcount[w.fresh[j]] = 1;
-    }
-    a.seq_lens[s] = len + a.other[i];
+    a.seq_lens[a.seqs[i]] = len + a.other[i];
+  }
+  for (int k = threadIdx.x; go && k < need; k += kPlanThreads) {
+    const int i = last_at_most(w.source, a.n, k);  // the request that page k is for
+    const int have = (int)(((int64_t)w.len[i] + page_mask) >> a.page_shift);
+    a.block_table[a.seqs[i] * a.table_stride + have + (k - w.source[i])] = w.fresh[k];
+    a.refcount[w.fresh[k]] = 1;
   }
   if (!go) report(a.status, bad ? kPagesBadIndex : longer ? kPagesTooLong : kPagesExhausted);
   if (threadIdx.x == 0) w.head[1] = go;
@@ -332,17 +355,13 @@ __global__ void __launch_bounds__(kCopyThreads) extend_slots(const PagesArgs a, 
                                                              int64_t* slots) {
   const PagesWork w = work_of(ws, a.n, most_pages);
   const int64_t t = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
+  wait_for_plan();
   if (t >= total_tokens) return;
   if (w.head[1] == 0) {
     slots[t] = -1;
     return;
   }
-  int lo = 0, hi = a.n - 1;  // the last request that starts at or before t, and is not empty
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (w.first[mid] <= t) lo = mid;
-    else hi = mid - 1;
-  }
+  const int lo = last_at_most(w.first, a.n, (int)t);  // the request that token t is of
   const int64_t pos = w.len[lo] + (t - w.first[lo]);
   const int pg = a.block_table[a.seqs[lo] * a.table_stride + (pos >> a.page_shift)];
   slots[t] = pg < 0 ? -1 : ((int64_t)pg << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
@@ -350,6 +369,7 @@ __global__ void __launch_bounds__(kCopyThreads) extend_slots(const PagesArgs a, 
 
 // ---- compact: the live pages above the live count move into the holes below it
 __global__ void __launch_bounds__(kPlanThreads) compact_plan(const PagesArgs a, int32_t* ws) {
+  launch_dependents();
   const PagesWork w = work_of(ws, 0, a.num_pages);
   int live = 0;
   for (int p = threadIdx.x; p < a.num_pages; p += kPlanThreads) live += a.refcount[p] != 0;
@@ -392,6 +412,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(const PagesArgs a, 
 __global__ void __launch_bounds__(kCopyThreads) compact_apply(const PagesArgs a, const PoolArgs c,
                                                               int32_t* ws) {
   const PagesWork w = work_of(ws, 0, a.num_pages);
+  wait_for_plan();
   const int pairs = w.head[0];
   if (pairs == 0) return;
   copy_pairs(c, w.source, w.target, pairs, blockIdx.x, gridDim.x);
@@ -410,6 +431,21 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply(const PagesArgs a,
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const PoolArgs c, const int32_t* source,
                                                             const int32_t* target, int64_t pairs) {
   copy_pairs(c, source, target, pairs, blockIdx.x, gridDim.x);
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_after_plan(void (*kernel)(Params...), unsigned grid, cudaStream_t stream,
+                              Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kCopyThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 PoolArgs with_chunks(PoolArgs c) {
@@ -436,8 +472,7 @@ cudaError_t launch_fork(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, i
   fork_plan<<<1, kPlanThreads, 0, stream>>>(a, ws);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  fork_apply<<<a.n + copy_grid(c, a.n, device_sms), kCopyThreads, 0, stream>>>(a, c, ws);
-  return cudaGetLastError();
+  return launch_after_plan(fork_apply, a.n + copy_grid(c, a.n, device_sms), stream, a, c, ws);
 }
 
 cudaError_t launch_free(const PagesArgs& a, cudaStream_t stream) {
@@ -450,9 +485,9 @@ cudaError_t launch_extend(const PagesArgs& a, int64_t total_tokens, int64_t most
   extend_plan<<<1, kPlanThreads, 0, stream>>>(a, total_tokens, most_pages, ws);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || total_tokens == 0) return e;
-  extend_slots<<<(unsigned)((total_tokens + kCopyThreads - 1) / kCopyThreads), kCopyThreads, 0,
-                 stream>>>(a, total_tokens, most_pages, ws, slots);
-  return cudaGetLastError();
+  return launch_after_plan(extend_slots,
+                           (unsigned)((total_tokens + kCopyThreads - 1) / kCopyThreads), stream, a,
+                           total_tokens, most_pages, ws, slots);
 }
 
 cudaError_t launch_compact(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, int device_sms,
@@ -461,8 +496,8 @@ cudaError_t launch_compact(const PagesArgs& a, const PoolArgs& pool, int32_t* ws
   compact_plan<<<1, kPlanThreads, 0, stream>>>(a, ws);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  compact_apply<<<copy_grid(c, a.num_pages / 2 + 1, device_sms), kCopyThreads, 0, stream>>>(a, c, ws);
-  return cudaGetLastError();
+  return launch_after_plan(compact_apply, copy_grid(c, a.num_pages / 2 + 1, device_sms), stream, a,
+                           c, ws);
 }
 
 cudaError_t launch_copy(const PoolArgs& pool, const int32_t* source, const int32_t* target,
