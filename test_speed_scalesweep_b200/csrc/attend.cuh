@@ -150,8 +150,8 @@ __device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype
   }
 }
 
-// Tiles of 256 rows on the tensor cores' own memory (kv_prompt.cu); head sizes 64 and 128.
-constexpr int kPromptRows = 256;
+// Long queries, on the tensor cores' own memory (kv_prompt.cu): rows of a tile.
+constexpr int prompt_rows(int head_size) { return head_size == 256 ? 128 : 256; }
 cudaError_t launch_prompt(const Params& p, cudaStream_t stream);
 
 }  // namespace kv

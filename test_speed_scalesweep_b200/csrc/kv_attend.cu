@@ -586,7 +586,8 @@ int log2i(int v) {
 
 // How one kernel cuts the batch.
 struct Cut {
-  int rows;  // of a tile; 0: not launched
+  int rows;    // of a tile; 0: not launched
+  int prompt;  // 1: the kernels of kv_prompt.cu
   int tiles, splits, chunk;
   int min_rows, max_rows;
 };
@@ -596,7 +597,7 @@ struct Plan {
 
 // `most` rows at most per sequence; `target` CTAs keep the GPU busy evenly.
 Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int64_t min_chunk) {
-  Cut c;
+  Cut c = {};
   c.rows = tile_rows;
   c.tiles = (int)((most + tile_rows - 1) / tile_rows);
   const int group = a.q_heads / a.cache.kv_heads;
@@ -605,7 +606,11 @@ Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int
   if (a.window >= 0 && span > (int64_t)a.window + tokens + kKeys)
     span = (int64_t)a.window + tokens + kKeys;
   const int64_t units = (int64_t)a.seqs * c.tiles * a.cache.kv_heads;
-  const int64_t splits = target / units < 1 ? 1 : target / units;
+  // Up to three stages per warp, a second launch costs more than the split
+  // saves (1 sequence of 300 keys: 8.2 us in one CTA per head, 9.2 split; of
+  // 700 keys 12.3 and 9.4).
+  const bool whole = target / units < 1 || (span <= 384 && tile_rows <= 8);
+  const int64_t splits = whole ? 1 : target / units;
   int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
   if (chunk < min_chunk) chunk = min_chunk;
   c.chunk = (int)chunk;
@@ -617,7 +622,10 @@ Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int
 Plan plan_of(const AttendArgs& a, int device_sms) {
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t rows = (int64_t)a.max_query_len * group;
-  const int most = a.cache.head_size == 256 ? 16 : 32;  // rows of decode_kernel's largest tile
+  // Rows up to which decode_kernel is the faster one (32 sequences of 8192 keys,
+  // 32 rows per kv head: heads of 64 198 us here, 224 on the tensor cores' own
+  // memory; heads of 128 331 and 262).
+  const int most = a.cache.head_size == 64 ? 32 : 16;
   // A single sequence is cut into one wave of CTAs (1 x 131072 keys, 8 kv heads:
   // 53 us with 3 CTAs per SM, 57 with 8, 70 with 12, each with a start and a
   // partial result of its own).  Sequences of several lengths are cut finer, so
@@ -625,12 +633,13 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
   // 111 with 12, 117 with 72).
   const int64_t target = (int64_t)device_sms * (a.seqs == 1 ? 3 : 24);
   Plan pl = {};
-  if (rows <= most || a.cache.head_size == 256) {
+  if (rows <= most) {
     pl.decode = cut_of(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, target, 128);
     pl.decode.max_rows = 0x7FFFFFFF;
     return pl;
   }
-  pl.prompt = cut_of(a, kPromptRows, rows, device_sms, 512);
+  pl.prompt = cut_of(a, prompt_rows(a.cache.head_size), rows, device_sms, 512);
+  pl.prompt.prompt = 1;
   pl.prompt.max_rows = 0x7FFFFFFF;
   if (a.seqs > 1) {  // single tokens among prompts
     pl.decode = cut_of(a, group <= 8 ? 8 : 16, 16, target, 128);
@@ -667,7 +676,7 @@ template <int kD>
 cudaError_t launch_rows(const Params& p, int rows, cudaStream_t stream) {
   if (rows == 8) return launch_decode<kD, 1>(p, stream);
   if (rows == 16) return launch_decode<kD, 2>(p, stream);
-  if constexpr (kD < 256) return launch_decode<kD, 4>(p, stream);
+  if constexpr (kD == 64) return launch_decode<kD, 4>(p, stream);
   return cudaErrorInvalidValue;
 }
 
@@ -695,10 +704,10 @@ cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
   p.min_rows = c.min_rows;
   p.max_rows = c.max_rows;
   const int d = p.a.cache.head_size;
-  cudaError_t e = c.rows == kPromptRows ? launch_prompt(p, stream)
-                  : d == 64             ? launch_rows<64>(p, c.rows, stream)
-                  : d == 128            ? launch_rows<128>(p, c.rows, stream)
-                                        : launch_rows<256>(p, c.rows, stream);
+  cudaError_t e = c.prompt   ? launch_prompt(p, stream)
+                  : d == 64  ? launch_rows<64>(p, c.rows, stream)
+                  : d == 128 ? launch_rows<128>(p, c.rows, stream)
+                             : launch_rows<256>(p, c.rows, stream);
   if (e != cudaSuccess || c.splits == 1) return e;
   return d == 64    ? launch_join<64>(p, c.rows, stream)
          : d == 128 ? launch_join<128>(p, c.rows, stream)

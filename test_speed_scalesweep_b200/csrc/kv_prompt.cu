@@ -46,6 +46,8 @@ constexpr int kMaskRing = 4;
 // whole row of S (128) and take what the others can spare:
 // 256 x 184 + 128 x 96 + 128 x 40 = 64512 of the launch's 65536.
 constexpr int kRegsSoftmax = 184, kRegsDequant = 96, kRegsMma = 40;
+// Heads of 256: 128 x 216 + 256 x 120 + 128 x 40 = 63488.
+constexpr int kRegsWideSoftmax = 216, kRegsWideDequant = 120;
 template <int kRegs>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -164,8 +166,8 @@ __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
 // Codes and scales of one key or value row.
 template <int kD>
 struct RowRegs {
-  uint32_t codes[kD / 8];
-  uint32_t scales[kD / 64];
+  alignas(16) uint32_t codes[kD / 8];
+  alignas(16) uint32_t scales[kD / 64];
 };
 
 template <int kD>
@@ -177,8 +179,10 @@ __device__ __forceinline__ void load_row(RowRegs<kD>& r, const uint8_t* codes,
       *reinterpret_cast<uint4*>(&r.codes[4 * j]) = __ldg(reinterpret_cast<const uint4*>(codes) + j);
     if constexpr (kD == 64) {
       r.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(scales));
-    } else {
+    } else if constexpr (kD == 128) {
       *reinterpret_cast<uint2*>(r.scales) = __ldg(reinterpret_cast<const uint2*>(scales));
+    } else {
+      *reinterpret_cast<uint4*>(r.scales) = __ldg(reinterpret_cast<const uint4*>(scales));
     }
   } else {  // what lies behind the last key may hold anything, NaN scales too
 #pragma unroll
@@ -204,6 +208,208 @@ __device__ __forceinline__ void store_row(const RowRegs<kD>& r, uint32_t tile, i
   }
 }
 
+// One softmax thread's row: its place, and the scale that turns scores into log2.
+struct Row {
+  bool live;
+  int64_t out_row;      // of lse and of the partial results
+  const uint16_t* src;  // of the query
+  uint16_t* dst;
+  int hi_key, lo_key;   // keys it sees
+  float scale;
+};
+
+__device__ __forceinline__ Row row_of(const Params& p, const Tile& tile, int head, int row_in) {
+  const AttendArgs& a = p.a;
+  Row w;
+  w.live = row_in < tile.rows;
+  const int row = tile.row0 + row_in, token = row / p.group, qh = head * p.group + row % p.group;
+  const int64_t at = tile.first_token + token;
+  w.out_row = at * a.q_heads + qh;
+  w.src = a.q.p + at * a.q.token_stride + (int64_t)qh * a.q.head_stride;
+  w.dst = a.out.p + at * a.out.token_stride + (int64_t)qh * a.out.head_stride;
+  const int pos = tile.offset + token;
+  w.hi_key = !w.live ? -1 : a.causal ? pos : 0x7FFFFFFF;
+  w.lo_key = a.window >= 0 ? pos - a.window : 0;
+  return w;
+}
+
+// The row of Q as f16, scaled as in decode_kernel, into the swizzled tile.
+template <int kD>
+__device__ __forceinline__ void load_query(const Params& p, Row& w, uint32_t tile, int r) {
+  const AttendArgs& a = p.a;
+  float scale = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  const bool flip = scale < 0.0f;  // the maximum is taken before scaling
+  scale = fabsf(scale);
+  float down = 1.0f;
+  if (a.dtype == kDTypeBF16 && w.live) {
+    uint32_t big = 0;
+#pragma unroll 4
+    for (int j = 0; j < kD / 8; ++j) {
+      const uint4 q = *(reinterpret_cast<const uint4*>(w.src) + j);
+      const uint32_t x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
+    }
+    const int e = (int)(big >> 23);
+    if (e >= 1 && e <= 253) {
+      down = __uint_as_float((uint32_t)(254 - e) << 23);
+      scale *= __uint_as_float((uint32_t)e << 23);
+    }
+  }
+  w.scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
+  if (flip) down = -down;
+#pragma unroll 4
+  for (int j = 0; j < kD / 8; ++j) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (w.live) {
+      q = *(reinterpret_cast<const uint4*>(w.src) + j);
+      uint32_t* x = reinterpret_cast<uint32_t*>(&q);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (a.dtype == kDTypeBF16)
+          x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
+                         __uint_as_float(x[c] & 0xFFFF0000u) * down);
+        else if (flip)
+          x[c] ^= 0x80008000u;
+      }
+    }
+    st_shared16(tile + tile_offset(r, j), q.x, q.y, q.z, q.w);
+  }
+}
+
+// Which keys of the block from k0 the row sees; false: all of them, for every
+// row of the warp.
+__device__ __forceinline__ bool block_mask(const Control* ctl, int j, int k0, const Row& w,
+                                           uint32_t (&mask)[4]) {
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    mask[x] = *reinterpret_cast<const volatile uint32_t*>(&ctl->mask[j % kMaskRing][x]);
+    const int first = k0 + 32 * x;
+    const int lo = w.lo_key - first, hi = w.hi_key - first;
+    const uint32_t above = lo <= 0 ? 0xFFFFFFFFu : lo > 31 ? 0u : 0xFFFFFFFFu << lo;
+    const uint32_t below = hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : 0xFFFFFFFFu >> (31 - hi);
+    mask[x] &= above & below;
+  }
+  return __any_sync(0xFFFFFFFFu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu);
+}
+
+// Softmax of the 128 scores at s_addr: updates the row's maximum and sum,
+// rescales O (kD columns at o_addr) where the maximum has grown by more than
+// the slack, and writes P over the scores.  `before_rescale` runs before O is
+// touched.
+template <int kD, typename F>
+__device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, bool masked,
+                                              const uint32_t (&mask)[4], float scale, bool first,
+                                              float& m, float& l, F&& before_rescale) {
+  uint32_t v[128];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
+  tmem_wait_ld();
+  if (masked) {
+#pragma unroll
+    for (int x = 0; x < 128; ++x)
+      if (!((mask[x / 32] >> (x % 32)) & 1u)) v[x] = 0xFF800000u;
+  }
+  float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int x = 0; x < 128; x += 8)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      top[y] = fmaxf(fmaxf(top[y], __uint_as_float(v[x + 2 * y])), __uint_as_float(v[x + 2 * y + 1]));
+  const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+  if (__any_sync(0xFFFFFFFFu, mx > m + kSlack)) {
+    const float mn = fmaxf(m, mx);
+    const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
+    m = mn;
+    l *= f;
+    if (!first) {  // nothing is in O before the first block
+      before_rescale();
+#pragma unroll 1
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_addr + 32 * c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+        tmem_st32(o_addr + 32 * c, o);
+      }
+    }
+  }
+  const float ms = m == -INFINITY ? 0.0f : m - kShift;
+  const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
+  uint64_t sums[2] = {0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w[16];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int at = 32 * c + 2 * x;
+      float e0, e1;
+      unpack2(fma2(pack2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), scale2, ms2), e0, e1);
+      const float p0 = ex2(e0), p1 = ex2(e1);
+      sums[x & 1] = add2(sums[x & 1], pack2(p0, p1));
+      w[x] = pack_h2(p0, p1);
+    }
+    tmem_st16(s_addr + 16 * c, w);
+  }
+  float sum[4];
+  unpack2(sums[0], sum[0], sum[1]);
+  unpack2(sums[1], sum[2], sum[3]);
+  l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+  asm volatile("tcgen05.fence::before_thread_sync;");
+}
+
+// The row's result from O (kD columns at o_addr): out, or a split's partial.
+template <int kD>
+__device__ __forceinline__ void store_result(const Params& p, const Row& w, int split,
+                                             uint32_t o_addr, bool any, float m, float l) {
+  const AttendArgs& a = p.a;
+  const bool seen = m != -INFINITY;  // a row that sees no key is zero
+  const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + w.out_row;
+  const float inv = seen ? (p.splits == 1 ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 1.0f) : 0.0f;
+#pragma unroll 1
+  for (int c = 0; c < kD / 32; ++c) {
+    uint32_t v[32];
+    if (any) {
+      tmem_ld32(o_addr + 32 * c, v);
+      tmem_wait_ld();
+    }
+    if (!w.live) continue;
+    float o[32];
+#pragma unroll
+    for (int x = 0; x < 32; ++x) o[x] = seen ? __uint_as_float(v[x]) * inv : 0.0f;
+    if (p.splits == 1) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        uint32_t h[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if (a.dtype == kDTypeBF16) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
+            h[y] = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            h[y] = pack_h2(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
+          }
+        }
+        *reinterpret_cast<uint4*>(w.dst + 32 * c + 8 * x) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        *reinterpret_cast<float4*>(p.part_o + part_row * kD + 32 * c + 4 * x) =
+            make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+    }
+  }
+  if (!w.live) return;
+  if (p.splits > 1)
+    *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
+  else if (a.lse)
+    a.lse[w.out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
+}
+
 template <int kD>
 __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   using S = PromptShape<kD>;
@@ -214,7 +420,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
   // the last tiles see the most keys: they start first
   Tile tile;
-  if (!tile_of(p, seq, p.tiles - 1 - blockIdx.x % p.tiles, kPromptRows, tile)) return;
+  if (!tile_of(p, seq, p.tiles - 1 - blockIdx.x % p.tiles, prompt_rows(kD), tile)) return;
   const int base = tile.beg & ~(kKeys - 1);
   if (split > 0 && base + (int64_t)split * p.chunk >= tile.end) return;
   const int c0 = base + split * p.chunk;
@@ -345,187 +551,30 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     }
   } else {
     more_registers<kRegsSoftmax>();
-    const int half = warp >> 2, r = (warp & 3) * 32 + lane, row_in = half * 128 + r;
-    const bool live = row_in < tile.rows;
-    const int row = tile.row0 + row_in, token = row / p.group, qh = head * p.group + row % p.group;
-    // ---- Q: this thread's row, scaled as in decode_kernel, into the swizzled tile
-    float scale = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
-    const bool flip = scale < 0.0f;  // the maximum below is taken before scaling
-    scale = fabsf(scale);
-    const uint16_t* src = a.q.p + (int64_t)(tile.first_token + token) * a.q.token_stride +
-                          (int64_t)qh * a.q.head_stride;
-    float down = 1.0f;
-    if (a.dtype == kDTypeBF16 && live) {
-      uint32_t big = 0;
-#pragma unroll 4
-      for (int j = 0; j < kD / 8; ++j) {
-        const uint4 w = *(reinterpret_cast<const uint4*>(src) + j);
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
-      }
-      const int e = (int)(big >> 23);
-      if (e >= 1 && e <= 253) {
-        down = __uint_as_float((uint32_t)(254 - e) << 23);
-        scale *= __uint_as_float((uint32_t)e << 23);
-      }
-    }
-    scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
-    if (flip) down = -down;
-#pragma unroll 4
-    for (int j = 0; j < kD / 8; ++j) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (live) {
-        w = *(reinterpret_cast<const uint4*>(src) + j);
-        uint32_t* x = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (a.dtype == kDTypeBF16)
-            x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
-                           __uint_as_float(x[c] & 0xFFFF0000u) * down);
-          else if (flip)
-            x[c] ^= 0x80008000u;
-        }
-      }
-      st_shared16(q_tile + half * S::kTile + tile_offset(r, j), w.x, w.y, w.z, w.w);
-    }
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    Row w = row_of(p, tile, head, half * 128 + r);
+    load_query<kD>(p, w, q_tile + half * S::kTile, r);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     bar_arrive(kBarQ, 256 + 32);
 
-    const int pos = tile.offset + token;
-    const int hi_key = !live ? -1 : a.causal ? pos : 0x7FFFFFFF;
-    const int lo_key = a.window >= 0 ? pos - a.window : 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + S::kS + 128 * half;
     const uint32_t o_addr = tmem + lanes + S::kO + kD * half;
     float m = -INFINITY, l = 0.0f;
     const bool work = half == 0 || two;
     for (int j = 0; work && j < blocks; ++j) {
-      const int k0 = c0 + j * kBlock;
       if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        mask[w] = *reinterpret_cast<volatile uint32_t*>(&ctl->mask[j % kMaskRing][w]);
-        // bits of keys lo_key .. hi_key
-        const int first = k0 + 32 * w;
-        const int lo = lo_key - first, hi = hi_key - first;
-        const uint32_t above = lo <= 0 ? 0xFFFFFFFFu : lo > 31 ? 0u : 0xFFFFFFFFu << lo;
-        const uint32_t below = hi >= 31 ? 0xFFFFFFFFu : hi < 0 ? 0u : 0xFFFFFFFFu >> (31 - hi);
-        mask[w] &= above & below;
-      }
-      const bool masked =
-          __any_sync(0xFFFFFFFFu, (mask[0] & mask[1] & mask[2] & mask[3]) != 0xFFFFFFFFu);
+      const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
       if (ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), j & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
-      uint32_t v[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(v + 32 * c));
-      tmem_wait_ld();
-      if (masked) {
-#pragma unroll
-        for (int x = 0; x < 128; ++x)
-          if (!((mask[x / 32] >> (x % 32)) & 1u)) v[x] = 0xFF800000u;
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int x = 0; x < 128; x += 8)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          top[y] = fmaxf(fmaxf(top[y], __uint_as_float(v[x + 2 * y])), __uint_as_float(v[x + 2 * y + 1]));
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
-      if (__any_sync(0xFFFFFFFFu, mx > m + kSlack)) {
-        const float mn = fmaxf(m, mx);
-        const float f = mn == -INFINITY ? 1.0f : ex2(m - mn);
-        m = mn;
-        l *= f;
-        if (j > 0) {  // nothing is in O before the first block
-#pragma unroll 1
-          for (int c = 0; c < kD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * c, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-            tmem_st32(o_addr + 32 * c, o);
-          }
-        }
-      }
-      const float ms = m == -INFINITY ? 0.0f : m - kShift;
-      const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
-      uint64_t sums[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int at = 32 * c + 2 * x;
-          float e0, e1;
-          unpack2(fma2(pack2(__uint_as_float(v[at]), __uint_as_float(v[at + 1])), scale2, ms2), e0, e1);
-          const float p0 = ex2(e0), p1 = ex2(e1);
-          sums[x & 1] = add2(sums[x & 1], pack2(p0, p1));
-          w[x] = pack_h2(p0, p1);
-        }
-        tmem_st16(s_addr + 16 * c, w);
-      }
-      float sum[4];
-      unpack2(sums[0], sum[0], sum[1]);
-      unpack2(sums[1], sum[2], sum[3]);
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      asm volatile("tcgen05.fence::before_thread_sync;");
+      // the P V before this S was issued before it, and has completed with it
+      softmax_block<kD>(s_addr, o_addr, masked, mask, w.scale, j == 0, m, l, [] {});
       bar_arrive(kBarP + half, 128 + 32);
     }
-    // ---- the row's result
     if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    const bool seen = m != -INFINITY;
-    const int64_t out_row = (int64_t)(tile.first_token + token) * a.q_heads + qh;
-    const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + out_row;
-    const float inv = seen ? (p.splits == 1 ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 1.0f) : 0.0f;
-    uint16_t* dst = a.out.p + (int64_t)(tile.first_token + token) * a.out.token_stride +
-                    (int64_t)qh * a.out.head_stride;
-#pragma unroll 1
-    for (int c = 0; c < kD / 32; ++c) {
-      uint32_t v[32];
-      if (work && blocks > 0) {
-        tmem_ld32(o_addr + 32 * c, v);
-        tmem_wait_ld();
-      }
-      if (!live) continue;
-      float o[32];
-#pragma unroll
-      for (int x = 0; x < 32; ++x) o[x] = seen ? __uint_as_float(v[x]) * inv : 0.0f;
-      if (p.splits == 1) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t w[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            if (a.dtype == kDTypeBF16) {
-              const __nv_bfloat162 h = __floats2bfloat162_rn(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
-              w[y] = *reinterpret_cast<const uint32_t*>(&h);
-            } else {
-              w[y] = pack_h2(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
-            }
-          }
-          *reinterpret_cast<uint4*>(dst + 32 * c + 8 * x) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      } else {
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-          *reinterpret_cast<float4*>(p.part_o + part_row * kD + 32 * c + 4 * x) =
-              make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
-      }
-    }
-    if (live) {
-      if (p.splits > 1)
-        *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
-      else if (a.lse)
-        a.lse[out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
-    }
+    store_result<kD>(p, w, split, o_addr, work && blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
@@ -534,6 +583,187 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     asm volatile("tcgen05.fence::after_thread_sync;");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
+}
+
+// Heads of 256: a tile of 128 rows, one K tile and one V tile of 64 KB beside
+// Q's, and two score buffers in TMEM beside O's 256 columns.  The next block's
+// Q K^T is issued before this block's P V, so that the softmax has both to hide
+// behind; K and V are dequantized by a warpgroup each, into the tile that the
+// tensor cores have just finished with.  Warps 0-3: softmax; 4-7: V; 8-11: K;
+// 12: MMAs.
+struct WideControl {
+  uint64_t s_full[2];  // scores are in buffer 0 / 1 (and K's tile is free)
+  uint64_t o_done;     // a P V has completed (and V's tile is free)
+};
+static_assert(sizeof(WideControl) <= sizeof(uint64_t) * 6, "fits in front of Control's masks");
+
+__global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params p) {
+  constexpr int kD = 256, kTile = 16384 * (kD / 64);
+  constexpr uint32_t kO = 256;  // TMEM: score buffers at 0 and 128, O from 256
+  constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kBlock >> 3) << 17) | (8u << 24);
+  constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kD >> 3) << 17) | (8u << 24);
+  constexpr int kBarK = kBarSlot, kBarV = kBarSlot + 1;
+  extern __shared__ uint8_t smem_raw[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
+  Tile tile;
+  if (!tile_of(p, seq, p.tiles - 1 - blockIdx.x % p.tiles, prompt_rows(kD), tile)) return;
+  const int base = tile.beg & ~(kKeys - 1);
+  if (split > 0 && base + (int64_t)split * p.chunk >= tile.end) return;
+  const int c0 = base + split * p.chunk;
+  const int c1 = (int)min((int64_t)tile.end, (int64_t)c0 + p.chunk);
+  const int blocks = c1 > c0 ? (c1 - c0 + kBlock - 1) / kBlock : 0;
+
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t q_tile = smem, k_tile = smem + kTile, v_tile = smem + 2 * kTile;
+  Control* ctl = reinterpret_cast<Control*>(smem_raw + (smem + 3 * kTile - smem_u32(smem_raw)));
+  WideControl* wide = reinterpret_cast<WideControl*>(ctl);  // over empty[] and s_full[]
+  const uint32_t s_full[2] = {smem_u32(&wide->s_full[0]), smem_u32(&wide->s_full[1])};
+  const uint32_t o_done = smem_u32(&wide->o_done);
+  if (threadIdx.x == 0) {
+    mbar_init(s_full[0], 1);
+    mbar_init(s_full[1], 1);
+    mbar_init(o_done, 1);
+    for (int i = 0; i < kMaskRing; ++i) mbar_init(smem_u32(&ctl->mask_full[i]), 4);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&ctl->tmem)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
+  bool ok = true;
+
+  if (warp >= kWarpMma) {
+    fewer_registers<kRegsMma>();
+    if (warp == kWarpMma) {
+      bar_sync(kBarQ, 128 + 32);
+      auto qk = [&](int j) {
+        bar_sync(kBarK, 128 + 32);
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < kD / 16; ++i) {
+            const uint32_t off = (i / 4) * 16384 + 32 * (i % 4);
+            mma_ss(tmem + 128 * (j & 1), smem_desc(q_tile + off, 16, 1024),
+                   smem_desc(k_tile + off, 16, 1024), kIdescQK, i != 0);
+          }
+          mma_commit(s_full[j & 1]);
+        }
+      };
+      if (blocks > 0) qk(0);
+      for (int j = 0; j < blocks; ++j) {
+        if (j + 1 < blocks) qk(j + 1);
+        bar_sync(kBarV, 128 + 32);
+        bar_sync(kBarP + (j & 1), 128 + 32);
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        if (lane == 0) {
+#pragma unroll
+          for (int i = 0; i < kBlock / 16; ++i)
+            mma_ts(tmem + kO, tmem + 128 * (j & 1) + 8 * i, smem_desc(v_tile + 2048 * i, 16384, 1024),
+                   kIdescPV, (j | i) != 0);
+          mma_commit(o_done);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    fewer_registers<kRegsWideDequant>();
+    const bool value = warp < kWarpDequant;
+    const int i = threadIdx.x & 127;  // this thread's key of a block
+    const int page_mask = (1 << p.page_shift) - 1;
+    const int32_t* table = a.block_table + (int64_t)seq * a.table_stride;
+    const int64_t side = value ? (int64_t)a.cache.kv_heads << p.page_shift : 0;
+    auto page_of = [&](int j) -> int {
+      const int key = c0 + j * kBlock + i;
+      if (key >= c1 || key < tile.beg) return -1;
+      const int pg = __ldg(table + (key >> p.page_shift));
+      return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
+    };
+    auto fetch = [&](RowRegs<kD>& r, int j, int pg) {
+      const int key = c0 + j * kBlock + i;
+      const int64_t row = side + ((int64_t)head << p.page_shift) + (key & page_mask);
+      load_row<kD>(r, a.cache.codes + pg * a.cache.codes_page_stride + row * (kD / 2),
+                   a.cache.scales + pg * a.cache.scales_page_stride + row * (kD / 16), pg >= 0);
+    };
+    RowRegs<kD> r;
+    int pg = page_of(0), pg_next = page_of(1);
+    fetch(r, 0, pg);
+    for (int j = 0; j < blocks; ++j) {
+      const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
+      if (j > 0 && ok)
+        ok = value ? mbar_wait(o_done, (j - 1) & 1)
+                   : mbar_wait(s_full[(j - 1) & 1], ((j - 1) >> 1) & 1);
+      if (!value && lane == 0) {
+        ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
+        mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
+      }
+      store_row<kD>(r, value ? v_tile : k_tile, i);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      bar_arrive(value ? kBarV : kBarK, 128 + 32);
+      pg = pg_next;
+      pg_next = page_of(j + 2);
+      fetch(r, j + 1, pg);
+    }
+  } else {
+    more_registers<kRegsWideSoftmax>();
+    const int r = threadIdx.x;
+    Row w = row_of(p, tile, head, r);
+    load_query<kD>(p, w, q_tile, r);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    bar_arrive(kBarQ, 128 + 32);
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < blocks; ++j) {
+      if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      uint32_t mask[4];
+      const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
+      if (ok) ok = mbar_wait(s_full[j & 1], (j >> 1) & 1);
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      // these scores were issued before the last P V, which O's rescaling must
+      // wait for
+      softmax_block<kD>(tmem + lanes + 128 * (j & 1), tmem + lanes + kO, masked, mask, w.scale,
+                        j == 0, m, l, [&] {
+                          if (ok) ok = mbar_wait(o_done, (j - 1) & 1);
+                          asm volatile("tcgen05.fence::after_thread_sync;");
+                        });
+      // The next scores may be there before this P V is issued, so the softmax
+      // can be one block ahead of the MMA warp: two barriers in turn.  It cannot
+      // be two ahead, the scores after the next being issued behind this P V.
+      bar_arrive(kBarP + (j & 1), 128 + 32);
+    }
+    // The last scores only tell that the P V two blocks before has completed: a
+    // parity wait may not skip the one between.
+    if (blocks > 1 && ok) ok = mbar_wait(o_done, (blocks - 2) & 1);
+    if (blocks > 0 && ok) ok = mbar_wait(o_done, (blocks - 1) & 1);
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    store_result<kD>(p, w, split, tmem + lanes + kO, blocks > 0, m, l);
+  }
+  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+cudaError_t launch_wide(const Params& p, cudaStream_t stream) {
+  constexpr int kSmem = 3 * 65536 + 256 + 1024;
+  const cudaError_t e = cudaFuncSetAttribute(prompt_wide_kernel,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
+  prompt_wide_kernel<<<grid, kPThreads, kSmem, stream>>>(p);
+  return cudaGetLastError();
 }
 
 template <int kD>
@@ -553,7 +783,7 @@ cudaError_t launch_d(const Params& p, cudaStream_t stream) {
 cudaError_t launch_prompt(const Params& p, cudaStream_t stream) {
   if (p.a.cache.head_size == 64) return launch_d<64>(p, stream);
   if (p.a.cache.head_size == 128) return launch_d<128>(p, stream);
-  return cudaErrorInvalidValue;
+  return launch_wide(p, stream);
 }
 
 }  // namespace kv
