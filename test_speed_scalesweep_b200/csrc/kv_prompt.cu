@@ -241,12 +241,15 @@ __device__ __forceinline__ void load_query(const Params& p, Row& w, uint32_t til
   const bool flip = scale < 0.0f;  // the maximum is taken before scaling
   scale = fabsf(scale);
   float down = 1.0f;
-  if (a.dtype == kDTypeBF16 && w.live) {
+  uint4 q[kD / 8];  // the whole row in flight at once
+#pragma unroll
+  for (int j = 0; j < kD / 8; ++j)
+    q[j] = w.live ? __ldg(reinterpret_cast<const uint4*>(w.src) + j) : make_uint4(0, 0, 0, 0);
+  if (a.dtype == kDTypeBF16) {
     uint32_t big = 0;
-#pragma unroll 4
+#pragma unroll
     for (int j = 0; j < kD / 8; ++j) {
-      const uint4 q = *(reinterpret_cast<const uint4*>(w.src) + j);
-      const uint32_t x[4] = {q.x, q.y, q.z, q.w};
+      const uint32_t x[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
@@ -259,22 +262,18 @@ __device__ __forceinline__ void load_query(const Params& p, Row& w, uint32_t til
   }
   w.scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
   if (flip) down = -down;
-#pragma unroll 4
-  for (int j = 0; j < kD / 8; ++j) {
-    uint4 q = make_uint4(0, 0, 0, 0);
-    if (w.live) {
-      q = *(reinterpret_cast<const uint4*>(w.src) + j);
-      uint32_t* x = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (a.dtype == kDTypeBF16)
-          x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
-                         __uint_as_float(x[c] & 0xFFFF0000u) * down);
-        else if (flip)
-          x[c] ^= 0x80008000u;
-      }
+  for (int j = 0; j < kD / 8; ++j) {
+    uint32_t* x = reinterpret_cast<uint32_t*>(&q[j]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (a.dtype == kDTypeBF16)
+        x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
+                       __uint_as_float(x[c] & 0xFFFF0000u) * down);
+      else if (flip)
+        x[c] ^= 0x80008000u;
     }
-    st_shared16(tile + tile_offset(r, j), q.x, q.y, q.z, q.w);
+    st_shared16(tile + tile_offset(r, j), q[j].x, q[j].y, q[j].z, q[j].w);
   }
 }
 
