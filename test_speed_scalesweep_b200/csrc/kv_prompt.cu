@@ -233,48 +233,65 @@ __device__ __forceinline__ Row row_of(const Params& p, const Tile& tile, int hea
   return w;
 }
 
-// The row of Q as f16, scaled as in decode_kernel, into the swizzled tile.
+// A pointer that lane `from` holds.
+template <typename T>
+__device__ __forceinline__ T* shfl_pointer(T* p, int from) {
+  return reinterpret_cast<T*>(
+      __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(p), from));
+}
+
+// The warp's 32 rows of Q as f16, scaled as in decode_kernel, into rows r0 ..
+// r0 + 31 of the swizzled tile.  Neighbouring lanes take neighbouring parts of
+// a row, and all loads are in flight at once (a row per thread, 16 bytes at a
+// time, took 8000 cycles for heads of 128).
 template <int kD>
-__device__ __forceinline__ void load_query(const Params& p, Row& w, uint32_t tile, int r) {
+__device__ __forceinline__ void load_queries(const Params& p, Row& w, uint32_t tile, int r0) {
+  constexpr int kLanes = kD / 8;           // lanes of a row
+  constexpr int kPer = 32 / kLanes;        // rows of a warp load
   const AttendArgs& a = p.a;
-  float scale = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
-  const bool flip = scale < 0.0f;  // the maximum is taken before scaling
-  scale = fabsf(scale);
-  float down = 1.0f;
-  uint4 q[kD / 8];  // the whole row in flight at once
+  const int lane = threadIdx.x & 31, part = lane % kLanes;
+  const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  const bool flip = signed_log2 < 0.0f;  // the maximum is taken before scaling
+  float scale = fabsf(signed_log2);
+  uint4 q[32 / kPer];
 #pragma unroll
-  for (int j = 0; j < kD / 8; ++j)
-    q[j] = w.live ? __ldg(reinterpret_cast<const uint4*>(w.src) + j) : make_uint4(0, 0, 0, 0);
-  if (a.dtype == kDTypeBF16) {
-    uint32_t big = 0;
+  for (int i = 0; i < 32 / kPer; ++i) {
+    const int row = i * kPer + lane / kLanes;
+    const uint16_t* src = shfl_pointer(w.src, row);
+    const bool live = __shfl_sync(0xFFFFFFFFu, (int)w.live, row);
+    q[i] = live ? __ldg(reinterpret_cast<const uint4*>(src) + part) : make_uint4(0, 0, 0, 0);
+  }
 #pragma unroll
-    for (int j = 0; j < kD / 8; ++j) {
-      const uint32_t x[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+  for (int i = 0; i < 32 / kPer; ++i) {
+    uint32_t* x = reinterpret_cast<uint32_t*>(&q[i]);
+    if (a.dtype == kDTypeBF16) {
+      uint32_t big = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
-    }
-    const int e = (int)(big >> 23);
-    if (e >= 1 && e <= 253) {
-      down = __uint_as_float((uint32_t)(254 - e) << 23);
-      scale *= __uint_as_float((uint32_t)e << 23);
-    }
-  }
-  w.scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
-  if (flip) down = -down;
 #pragma unroll
-  for (int j = 0; j < kD / 8; ++j) {
-    uint32_t* x = reinterpret_cast<uint32_t*>(&q[j]);
+      for (int o = 1; o < kLanes; o <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+      const int e = (int)(big >> 23);
+      const bool sized = e >= 1 && e <= 253;
+      const float size = sized ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
+      const float down = flip ? -size : size;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (a.dtype == kDTypeBF16)
+      for (int c = 0; c < 4; ++c)
         x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
                        __uint_as_float(x[c] & 0xFFFF0000u) * down);
-      else if (flip)
-        x[c] ^= 0x80008000u;
+      // the row's own thread keeps what the scores have to be multiplied by
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int ek = __shfl_sync(0xFFFFFFFFu, sized ? e : 127, k * kLanes);
+        if (lane == i * kPer + k) scale *= __uint_as_float((uint32_t)ek << 23);
+      }
+    } else if (flip) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] ^= 0x80008000u;
     }
-    st_shared16(tile + tile_offset(r, j), q[j].x, q[j].y, q[j].z, q[j].w);
+    st_shared16(tile + tile_offset(r0 + i * kPer + lane / kLanes, part), x[0], x[1], x[2], x[3]);
   }
+  w.scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
 }
 
 // Which keys of the block from k0 the row sees; false: all of them, for every
@@ -361,52 +378,82 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
   asm volatile("tcgen05.fence::before_thread_sync;");
 }
 
-// The row's result from O (kD columns at o_addr): out, or a split's partial.
+// 128 bytes of each of the warp's 32 rows, held a row per thread, to `dst` (each
+// thread's own row, null: none), through 4 KB of shared memory: eight lanes
+// store a row's 128 bytes (16 bytes per row and instruction took 7000 cycles
+// for a tile of heads of 128).
+__device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[32], uint8_t* dst) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    st_shared16(stage + lane * 128 + (((c ^ lane) & 7) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2],
+                v[4 * c + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = 4 * i + (lane >> 3), c = lane & 7;
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(stage + row * 128 + (((c ^ row) & 7) << 4))
+                 : "memory");
+    uint8_t* to = shfl_pointer(dst, row);
+    if (to) *reinterpret_cast<uint4*>(to + 16 * c) = x;
+  }
+  __syncwarp();
+}
+
+// The rows' results from O (kD columns at o_addr): out, or a split's partial.
+// `stage`: 4 KB of shared memory of the warp's own.
 template <int kD>
 __device__ __forceinline__ void store_result(const Params& p, const Row& w, int split,
-                                             uint32_t o_addr, bool any, float m, float l) {
+                                             uint32_t o_addr, uint32_t stage, bool any, float m,
+                                             float l) {
   const AttendArgs& a = p.a;
-  const bool seen = m != -INFINITY;  // a row that sees no key is zero
+  const bool seen = any && m != -INFINITY;  // a row that sees no key is zero
   const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + w.out_row;
-  const float inv = seen ? (p.splits == 1 ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 1.0f) : 0.0f;
+  if (p.splits == 1) {
+    const float inv = seen ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 0.0f;
 #pragma unroll 1
-  for (int c = 0; c < kD / 32; ++c) {
-    uint32_t v[32];
-    if (any) {
-      tmem_ld32(o_addr + 32 * c, v);
-      tmem_wait_ld();
-    }
-    if (!w.live) continue;
-    float o[32];
+    for (int c = 0; c < kD / 64; ++c) {
+      uint32_t h[32];
 #pragma unroll
-    for (int x = 0; x < 32; ++x) o[x] = seen ? __uint_as_float(v[x]) * inv : 0.0f;
-    if (p.splits == 1) {
+      for (int k = 0; k < 2; ++k) {
+        uint32_t v[32];
+        if (any) {
+          tmem_ld32(o_addr + 64 * c + 32 * k, v);
+          tmem_wait_ld();
+        }
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t h[4];
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
+        for (int x = 0; x < 16; ++x) {
+          const float lo = seen ? __uint_as_float(v[2 * x]) * inv : 0.0f;
+          const float hi = seen ? __uint_as_float(v[2 * x + 1]) * inv : 0.0f;
           if (a.dtype == kDTypeBF16) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
-            h[y] = *reinterpret_cast<const uint32_t*>(&b);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+            h[16 * k + x] = *reinterpret_cast<const uint32_t*>(&b);
           } else {
-            h[y] = pack_h2(o[8 * x + 2 * y], o[8 * x + 2 * y + 1]);
+            h[16 * k + x] = pack_h2(lo, hi);
           }
         }
-        *reinterpret_cast<uint4*>(w.dst + 32 * c + 8 * x) = make_uint4(h[0], h[1], h[2], h[3]);
       }
-    } else {
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        *reinterpret_cast<float4*>(p.part_o + part_row * kD + 32 * c + 4 * x) =
-            make_float4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+      store_rows(stage, h, w.live ? reinterpret_cast<uint8_t*>(w.dst + 64 * c) : nullptr);
     }
+    if (w.live && a.lse) a.lse[w.out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+      uint32_t v[32];
+      if (any) {
+        tmem_ld32(o_addr + 32 * c, v);
+        tmem_wait_ld();
+      }
+#pragma unroll
+      for (int x = 0; x < 32; ++x) v[x] = seen ? v[x] : 0;
+      store_rows(stage, v,
+                 w.live ? reinterpret_cast<uint8_t*>(p.part_o + part_row * kD + 32 * c) : nullptr);
+    }
+    if (w.live) *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
   }
-  if (!w.live) return;
-  if (p.splits > 1)
-    *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
-  else if (a.lse)
-    a.lse[w.out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
 }
 
 template <int kD>
@@ -552,7 +599,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     more_registers<kRegsSoftmax>();
     const int half = warp >> 2, r = (warp & 3) * 32 + lane;
     Row w = row_of(p, tile, head, half * 128 + r);
-    load_query<kD>(p, w, q_tile + half * S::kTile, r);
+    load_queries<kD>(p, w, q_tile + half * S::kTile, (warp & 3) * 32);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     bar_arrive(kBarQ, 256 + 32);
 
@@ -573,7 +620,9 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     }
     if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    store_result<kD>(p, w, split, o_addr, work && blocks > 0, m, l);
+    // this half's MMAs are done with its Q, which becomes the staging area
+    store_result<kD>(p, w, split, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
+                     work && blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
@@ -716,7 +765,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     more_registers<kRegsWideSoftmax>();
     const int r = threadIdx.x;
     Row w = row_of(p, tile, head, r);
-    load_query<kD>(p, w, q_tile, r);
+    load_queries<kD>(p, w, q_tile, warp * 32);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     bar_arrive(kBarQ, 128 + 32);
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
@@ -744,7 +793,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     if (blocks > 1 && ok) ok = mbar_wait(o_done, (blocks - 2) & 1);
     if (blocks > 0 && ok) ok = mbar_wait(o_done, (blocks - 1) & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    store_result<kD>(p, w, split, tmem + lanes + kO, blocks > 0, m, l);
+    store_result<kD>(p, w, split, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
