@@ -157,6 +157,12 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
                "r"(d)
                : "memory");
 }
+__device__ __forceinline__ void ld_shared16(uint32_t addr, uint32_t (&x)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+               : "r"(addr)
+               : "memory");
+}
 // Byte offset of 16-byte chunk c of row r in a 128-row tile of 64-wide halves,
 // 128-byte swizzle: K-major for Q and K, N-major for V.
 __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
@@ -241,55 +247,68 @@ __device__ __forceinline__ T* shfl_pointer(T* p, int from) {
 }
 
 // The warp's 32 rows of Q as f16, scaled as in decode_kernel, into rows r0 ..
-// r0 + 31 of the swizzled tile.  Neighbouring lanes take neighbouring parts of
-// a row, and all loads are in flight at once (a row per thread, 16 bytes at a
-// time, took 8000 cycles for heads of 128).
+// r0 + 31 of the swizzled tile.  Asynchronous copies bring them, neighbouring
+// lanes neighbouring parts of a row; then each thread turns its own row over in
+// place.  Short loops: this code runs once per CTA, mostly from a cold
+// instruction cache.
 template <int kD>
 __device__ __forceinline__ void load_queries(const Params& p, Row& w, uint32_t tile, int r0) {
-  constexpr int kLanes = kD / 8;           // lanes of a row
-  constexpr int kPer = 32 / kLanes;        // rows of a warp load
+  constexpr int kLanes = kD / 8;     // lanes of a row
+  constexpr int kPer = 32 / kLanes;  // rows of a warp's copy
   const AttendArgs& a = p.a;
   const int lane = threadIdx.x & 31, part = lane % kLanes;
+  const uint16_t* const mine = w.live ? w.src : nullptr;
+#pragma unroll 2
+  for (int i = lane / kLanes; i < 32; i += kPer) {
+    const uint16_t* src = shfl_pointer(mine, i);
+    const uint32_t bytes = src ? 16 : 0;  // zeros for a row that is not there
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     tile + tile_offset(r0 + i, part)),
+                 "l"((src ? src : a.q.p) + part * 8), "r"(bytes)
+                 : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
   const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
   const bool flip = signed_log2 < 0.0f;  // the maximum is taken before scaling
   float scale = fabsf(signed_log2);
-  uint4 q[32 / kPer];
-#pragma unroll
-  for (int i = 0; i < 32 / kPer; ++i) {
-    const int row = i * kPer + lane / kLanes;
-    const uint16_t* src = shfl_pointer(w.src, row);
-    const bool live = __shfl_sync(0xFFFFFFFFu, (int)w.live, row);
-    q[i] = live ? __ldg(reinterpret_cast<const uint4*>(src) + part) : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int i = 0; i < 32 / kPer; ++i) {
-    uint32_t* x = reinterpret_cast<uint32_t*>(&q[i]);
-    if (a.dtype == kDTypeBF16) {
-      uint32_t big = 0;
+  if (a.dtype == kDTypeBF16) {
+    uint32_t big = 0;
+#pragma unroll 4
+    for (int j = 0; j < kD / 8; ++j) {
+      uint32_t x[4];
+      ld_shared16(tile + tile_offset(r0 + lane, j), x);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) big = max(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
-      const int e = (int)(big >> 23);
-      const bool sized = e >= 1 && e <= 253;
-      const float size = sized ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.0f;
-      const float down = flip ? -size : size;
+    }
+    const int e = (int)(big >> 23);
+    float down = 1.0f;
+    if (e >= 1 && e <= 253) {
+      down = __uint_as_float((uint32_t)(254 - e) << 23);
+      scale *= __uint_as_float((uint32_t)e << 23);
+    }
+    if (flip) down = -down;
+#pragma unroll 4
+    for (int j = 0; j < kD / 8; ++j) {
+      uint32_t x[4];
+      const uint32_t at = tile + tile_offset(r0 + lane, j);
+      ld_shared16(at, x);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
                        __uint_as_float(x[c] & 0xFFFF0000u) * down);
-      // the row's own thread keeps what the scores have to be multiplied by
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int ek = __shfl_sync(0xFFFFFFFFu, sized ? e : 127, k * kLanes);
-        if (lane == i * kPer + k) scale *= __uint_as_float((uint32_t)ek << 23);
-      }
-    } else if (flip) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] ^= 0x80008000u;
+      st_shared16(at, x[0], x[1], x[2], x[3]);
     }
-    st_shared16(tile + tile_offset(r0 + i * kPer + lane / kLanes, part), x[0], x[1], x[2], x[3]);
+  } else if (flip) {
+#pragma unroll 1
+    for (int j = 0; j < kD / 8; ++j) {
+      uint32_t x[4];
+      const uint32_t at = tile + tile_offset(r0 + lane, j);
+      ld_shared16(at, x);
+      st_shared16(at, x[0] ^ 0x80008000u, x[1] ^ 0x80008000u, x[2] ^ 0x80008000u,
+                  x[3] ^ 0x80008000u);
+    }
   }
   w.scale = fmaxf(scale, 1e-37f);  // never zero, or a masked score would be NaN
 }
@@ -392,13 +411,10 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[3
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = 4 * i + (lane >> 3), c = lane & 7;
-    uint4 x;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                 : "r"(stage + row * 128 + (((c ^ row) & 7) << 4))
-                 : "memory");
+    uint32_t x[4];
+    ld_shared16(stage + row * 128 + (((c ^ row) & 7) << 4), x);
     uint8_t* to = shfl_pointer(dst, row);
-    if (to) *reinterpret_cast<uint4*>(to + 16 * c) = x;
+    if (to) *reinterpret_cast<uint4*>(to + 16 * c) = make_uint4(x[0], x[1], x[2], x[3]);
   }
   __syncwarp();
 }
