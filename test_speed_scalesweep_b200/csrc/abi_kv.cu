@@ -199,6 +199,11 @@ int attend_args(const char* name, const ssw_kv_cache* cache, const ssw_kv_attent
     return fail(SSW_ERR_INVALID_ARGUMENT,
                 "%s: max_query_len and max_seq_len must be positive and below 2^30 rows (got %d, %d)",
                 name, x->max_query_len, x->max_seq_len);
+  // a launch has a CTA column per sequence and 8 rows of the longest query
+  if ((int64_t)x->seqs * ((int64_t)x->max_query_len * (x->q_heads / cache->kv_heads) / 8 + 1) >=
+      (1ll << 31))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: %d sequences of up to %d queries are too many", name,
+                x->seqs, x->max_query_len);
   if (x->block_table_columns < 1 || x->block_table_stride < x->block_table_columns)
     return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad block table (%d columns, stride %lld)", name,
                 x->block_table_columns, (long long)x->block_table_stride);

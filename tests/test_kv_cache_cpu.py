@@ -130,7 +130,7 @@ def attention(dtype=0, c=None, **kw):
     (dict(tokens=-1), "bad sizes"), (dict(tokens=1 << 40), "bad sizes"), (dict(seqs=-1), "bad sizes"),
     (dict(max_query_len=0), "max_query_len"), (dict(max_seq_len=0), "max_query_len"),
     (dict(max_seq_len=(1 << 30) + 1), "max_query_len"), (dict(max_query_len=1 << 30), "max_query_len"),
-    (dict(block_table_columns=0), "block table"), (dict(block_table_stride=3), "block table"),
+    (dict(seqs=1 << 30, max_query_len=1 << 20), "too many"), (dict(block_table_columns=0), "block table"), (dict(block_table_stride=3), "block table"),
     (dict(softmax_scale=math.inf), "finite"), (dict(softmax_scale=math.nan), "finite"),
     (dict(block_table=None), "null"), (dict(seq_lens=None), "null"), (dict(query_start=0x3002), "misaligned"),
     (dict(dtype=5), "dtype"), (dict(c=cache(head_size=192)), "head_size")])
