@@ -375,7 +375,8 @@ int ssw_nvfp4_kv_gather(const ssw_kv_cache* cache, int dtype, int64_t tokens,
  * out[r] = sum_j softmax_j(softmax_scale * q[r] . K[j]) V[j]; query head h uses
  * kv head h / (q_heads / kv_heads).  lse (may be null): float [tokens,
  * q_heads], the natural log of the sum of exp(softmax_scale * q . K).
- * max_query_len and max_seq_len bound the batch's lengths from above.
+ * max_query_len and max_seq_len bound the batch's lengths from above; queries
+ * and keys past them may be passed over.
  * status (may be null): an int set to 1 if a bounded device-side wait gave up
  * (the output is then undefined).
  */

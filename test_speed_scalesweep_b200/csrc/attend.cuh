@@ -135,10 +135,11 @@ __device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int 
   return true;
 }
 
-// Splits of a tile that hold keys (at least one, which then writes zeros).
+// Splits of a tile that hold keys (at least one, which then writes zeros).  A
+// sequence longer than the caller's max_seq_len has no more than were launched.
 __device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
   const int n = t.end - (t.beg & ~(kKeys - 1));
-  return max(1, (n + p.chunk - 1) / p.chunk);
+  return min(max(1, (n + p.chunk - 1) / p.chunk), p.splits);
 }
 
 __device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype) {  // 2 values

@@ -515,6 +515,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const int head = blockIdx.z, seq = blockIdx.x / p.tiles, r = blockIdx.y;
   __shared__ float part[kWarps][kD];
   __shared__ float part_m[kWarps], part_l[kWarps];
+  // every CTA waits, so that this grid does not end before the one it depends on
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Tile tile;
   if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) return;
   const int splits = used_splits(p, tile);
@@ -525,7 +527,6 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
   const float* po = p.part_o + out_row * kD + lane * kPer;
   const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   float mm = -INFINITY;
   for (int s = warp + lane * kWarps; s < splits; s += 32 * kWarps) mm = fmaxf(mm, ml[s * step].x);
 #pragma unroll

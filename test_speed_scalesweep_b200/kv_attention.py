@@ -26,7 +26,8 @@ def nvfp4_paged_attention(query: torch.Tensor, codes: torch.Tensor, scales: torc
     rows ``query_start[b]:query_start[b + 1]``.  ``block_table`` int32 [B, P]:
     its pages; an entry outside the cache (-1) holds no keys.
     ``max_query_len`` and ``max_seq_len`` bound the lengths from above; they size
-    the launch, so that nothing is read back.
+    the launch, so that nothing is read back.  Queries and keys past them may be
+    passed over.
 
     ``causal``: a query sees the keys up to its own position, its sequence's
     queries being the last of its keys.  ``window``: only those at most

@@ -14,6 +14,8 @@ from __future__ import annotations
 import torch
 
 from . import act_quant
+from . import kv_attention
+from . import kv_cache
 from . import norm_quant
 from . import scalesweep_mse_nvfp4_utils as mse
 from . import scalesweep_mse_reference_nvfp4_utils as mse_ref
@@ -95,6 +97,7 @@ def _register(namespace: str, kind: str) -> None:
         _register_act_quant(lib, namespace)
         _register_norm_quant(lib, namespace)
         _register_linear(lib, namespace)
+        _register_kv(lib, namespace)
     _libs[namespace] = lib
 
 
@@ -202,6 +205,49 @@ def _register_norm_quant(lib: torch.library.Library, namespace: str) -> None:
     torch.library.register_fake(f"{namespace}::{fn}", fake_functional, lib=lib)
     torch.library.register_fake(f"{namespace}::rms_norm_nvfp4_quant", fake_none, lib=lib)
     torch.library.register_fake(f"{namespace}::fused_add_rms_norm_nvfp4_quant", fake_none, lib=lib)
+
+
+def _register_kv(lib: torch.library.Library, namespace: str) -> None:
+    """The NVFP4 KV cache's operators of a model's forward pass (kv_cache.py,
+    kv_attention.py): the cache tensors are mutated by the write and only read
+    by the others."""
+    write, gather, attend = ("rotary_scalesweep_mse_nvfp4_kv_write", "nvfp4_kv_gather",
+                             "nvfp4_paged_attention")
+    lib.define(write + "(Tensor query, Tensor key, Tensor value, Tensor positions, "
+               "Tensor cos_sin_cache, Tensor slot_mapping, Tensor kv_input_scale, "
+               "Tensor(a!) codes, Tensor(b!) scales, bool is_neox=True) -> Tensor")
+    lib.define(gather + "(Tensor codes, Tensor scales, Tensor kv_input_scale, Tensor slot_mapping, "
+               "ScalarType dtype) -> (Tensor, Tensor)")
+    lib.define(attend + "(Tensor query, Tensor codes, Tensor scales, Tensor kv_input_scale, "
+               "Tensor block_table, Tensor seq_lens, Tensor query_start, SymInt max_query_len, "
+               "SymInt max_seq_len, float? softmax_scale=None, bool causal=True, "
+               "SymInt? window=None) -> Tensor")
+
+    def kv_write(query, key, value, positions, cos_sin_cache, slot_mapping, kv_input_scale, codes,
+                 scales, is_neox=True):
+        return kv_cache.rotary_scalesweep_mse_nvfp4_kv_write(
+            query, key, value, positions, cos_sin_cache, slot_mapping, kv_input_scale, codes, scales,
+            is_neox=is_neox)
+
+    def paged_attention(query, codes, scales, kv_input_scale, block_table, seq_lens, query_start,
+                        max_query_len, max_seq_len, softmax_scale=None, causal=True, window=None):
+        return kv_attention.nvfp4_paged_attention(
+            query, codes, scales, kv_input_scale, block_table, seq_lens, query_start, max_query_len,
+            max_seq_len, softmax_scale=softmax_scale, causal=causal, window=window)
+
+    def fake_like_query(query, *args, **kwargs):
+        return query.new_empty(query.shape)
+
+    def fake_gather(codes, scales, kv_input_scale, slot_mapping, dtype):
+        shape = (slot_mapping.shape[0], codes.shape[2], codes.shape[4] * 2)
+        return codes.new_empty(shape, dtype=dtype), codes.new_empty(shape, dtype=dtype)
+
+    lib.impl(write, kv_write, "CUDA")
+    lib.impl(gather, kv_cache.nvfp4_kv_gather, "CUDA")
+    lib.impl(attend, paged_attention, "CUDA")
+    torch.library.register_fake(f"{namespace}::{write}", fake_like_query, lib=lib)
+    torch.library.register_fake(f"{namespace}::{gather}", fake_gather, lib=lib)
+    torch.library.register_fake(f"{namespace}::{attend}", fake_like_query, lib=lib)
 
 
 def register() -> None:

@@ -240,3 +240,15 @@ def test_status_stays_clear(attn):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     b.call(attn, status=status)
     assert status.item() == 0
+
+
+@pytest.mark.parametrize("lens", [[(9000, 1)], [(9000, 1), (500, 1)], [(9000, 40)], [(5000, 300), (9000, 1)]])
+def test_bounds_smaller_than_the_batch_stay_in_bounds(attn, lens):
+    """Lengths past the bounds are passed over; the queries within them still look at the keys within them."""
+    b = Batch(lens, 4, 1, 128, 16, "bf16", seed=3)
+    guard = torch.full((b.q.shape[0], 4, 128), 5.0, dtype=torch.bfloat16, device="cuda")
+    for max_q, max_s in ((b.max_q, 700), (1, 9000), (1, 1)):
+        out = attn.nvfp4_paged_attention(b.q, b.codes, b.scales, b.mult, b.table, b.seq_lens, b.start, max_q,
+                                         max_s, out=guard.clone())
+        assert bool(out[0].isfinite().all()) and bool((out[0] != 5).any())
+    b.check(b.call(attn))

@@ -310,3 +310,27 @@ def test_a_serving_run(pages, dtype):
     step([0, 3, 4, 5], [1, 60, 2, 1])
     step([2, 1], [100, 1])
     step([0, 1, 2, 3, 4, 5], [1] * 6)
+
+
+def test_torch_ops_and_a_compiled_layer(pages):
+    """The registered ops give the functions' results, in a compiled graph too."""
+    from test_speed_scalesweep_b200 import kv_attention, kv_cache, ops  # noqa: F401
+    ns = torch.ops.scalesweep_b200
+    hq, hkv, d, n = 4, 2, 64, 33
+    table, mult = kv_cache.rotary_cos_sin_cache(64, d), torch.tensor([100.0, 120.0], device="cuda")
+    qkv = torch.randn(n, hq + 2 * hkv, d, device="cuda", generator=torch.Generator("cuda").manual_seed(0)).bfloat16()
+    idx, rows = torch.arange(n, device="cuda"), i32([[2, 0, 1]])
+
+    def layer(x, codes, scales):
+        q = ns.rotary_scalesweep_mse_nvfp4_kv_write(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], idx, table,
+                                                    slots, mult, codes, scales, True)
+        return ns.nvfp4_paged_attention(q, codes, scales, mult, rows, i32([n]), i32([0, n]), n, n) * 2
+
+    slots = rows[0, idx // 16].long() * 16 + idx % 16
+    caches = [kv_cache.alloc_kv_cache(3, 16, hkv, d) for _ in range(2)]
+    want = layer(qkv, *caches[0])
+    got = torch.compile(layer, backend="aot_eager", fullgraph=True)(qkv, *caches[1])
+    assert torch.equal(got, want) and torch.equal(caches[0][0][:, :, :, :1], caches[1][0][:, :, :, :1])
+    k, v = ns.nvfp4_kv_gather(*caches[0], mult, slots, torch.float16)
+    fk, fv = kv_cache.nvfp4_kv_gather(*caches[1], mult, slots, torch.float16)
+    assert torch.equal(k, fk) and torch.equal(v, fv)

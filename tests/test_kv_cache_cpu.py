@@ -199,3 +199,19 @@ def test_pages_python_refusals(built_library):
         kv_pages.NVFP4KVPages.empty(codes[0, 0], scales[0, 0], 2, 2)
     with pytest.raises(ValueError, match="head_size/16"):
         kv_pages.NVFP4KVPages.empty(codes, scales[..., :2], 2, 2)
+
+
+def test_ops_registered_with_fake_shapes():
+    from test_speed_scalesweep_b200 import ops  # noqa: F401
+    ns = torch.ops.scalesweep_b200
+    codes, scales = kv_cache.alloc_kv_cache(8, 16, 2, 128, device="meta")
+    q = torch.empty(5, 4, 128, dtype=torch.bfloat16, device="meta")
+    kv = torch.empty(5, 2, 128, dtype=torch.bfloat16, device="meta")
+    idx, mult = torch.empty(5, dtype=torch.int64, device="meta"), torch.empty(2, device="meta")
+    table = torch.empty(64, 128, device="meta")
+    out = ns.rotary_scalesweep_mse_nvfp4_kv_write(q, kv, kv, idx, table, idx, mult, codes, scales, True)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    i32 = [torch.empty(s, dtype=torch.int32, device="meta") for s in ((1, 4), (1,), (2,))]
+    assert ns.nvfp4_paged_attention(q, codes, scales, mult, *i32, 5, 64).shape == q.shape
+    k, v = ns.nvfp4_kv_gather(codes, scales, mult, idx, torch.float16)
+    assert k.shape == v.shape == (5, 2, 128) and k.dtype == torch.float16
