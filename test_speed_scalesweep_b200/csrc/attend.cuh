@@ -26,6 +26,7 @@ struct Params {
   int tiles;       // row tiles of the longest query
   int min_rows, max_rows;  // sequences with other numbers of rows are another kernel's
   int splits;      // CTAs that share a tile's keys
+  int beside;      // 1: decode_kernel launched while a prompt kernel may still run
   int chunk;       // keys of a split, a multiple of 128
   int page_shift;
   float* part_o;   // [split][row of q and head][head_size]

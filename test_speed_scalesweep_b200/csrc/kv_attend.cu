@@ -66,14 +66,13 @@ struct Flag {
 };
 
 template <int kD, int kNT>
-__global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1) decode_kernel(const Params p) {
+__device__ __forceinline__ void decode_tile(const Params& p) {
   using S = Shape<kD>;
   constexpr int kRows = kNT * 8;
   constexpr int kQuarter = kD / 4;             // elements of a key row per thread
   constexpr int kKWords = kD / 32;             // 32-bit words of codes per thread and key row
   constexpr int kVWords = kD / 64 < 1 ? 1 : kD / 64;  // words of codes per thread and value row
   extern __shared__ __align__(128) uint8_t smem[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.y, head = blockIdx.z;
@@ -504,21 +503,35 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1) decod
   }
 }
 
+template <int kD, int kNT>
+__global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
+    decode_kernel(const Params p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+  decode_tile<kD, kNT>(p);
+  // Beside a prompt kernel, which this grid does not read from: it ends after
+  // that one all the same, so that what follows finds both done.
+  if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // Joins the splits of one row, always in the same order: warp w takes splits w,
 // w + 4, ..., then the warps' results are joined.  A programmatic dependent of
 // the kernel that wrote them.
+constexpr int kJoinWarps = 4, kJoinThreads = kJoinWarps * 32;
 template <int kD>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int tile_rows) {
   constexpr int kPer = kD / 32;  // elements of a lane
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.z, seq = blockIdx.x / p.tiles, r = blockIdx.y;
-  __shared__ float part[kWarps][kD];
-  __shared__ float part_m[kWarps], part_l[kWarps];
-  // every CTA waits, so that this grid does not end before the one it depends on
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float part[kJoinWarps][kD];
+  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
+  // Everything that does not read the other grid's results comes before the
+  // wait; CTAs without a row wait too, so that this grid does not end first.
   Tile tile;
-  if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) return;
+  if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int splits = used_splits(p, tile);
   const int row = tile.row0 + r, token = tile.first_token + row / p.group;
   const int qh = head * p.group + row % p.group;
@@ -527,15 +540,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
   const float* po = p.part_o + out_row * kD + lane * kPer;
   const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float mm = -INFINITY;
-  for (int s = warp + lane * kWarps; s < splits; s += 32 * kWarps) mm = fmaxf(mm, ml[s * step].x);
+  for (int s = warp + lane * kJoinWarps; s < splits; s += 32 * kJoinWarps) mm = fmaxf(mm, ml[s * step].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
   float sum = 0.0f, acc[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
 #pragma unroll 4
-  for (int s = warp; s < splits; s += kWarps) {
+  for (int s = warp; s < splits; s += kJoinWarps) {
     const float2 x = ml[s * step];
     float v[kPer];
 #pragma unroll
@@ -555,19 +569,19 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   __syncthreads();
   float all = part_m[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) all = fmaxf(all, part_m[w]);
-  float f[kWarps], total = 0.0f;
+  for (int w = 1; w < kJoinWarps; ++w) all = fmaxf(all, part_m[w]);
+  float f[kJoinWarps], total = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kJoinWarps; ++w) {
     f[w] = all == -INFINITY ? 0.0f : ex2(part_m[w] - all);
     total += f[w] * part_l[w];
   }
   const float inv = all == -INFINITY ? 0.0f : inv_mult / total;
   uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
-  for (int d = threadIdx.x * 2; d < kD; d += kThreads * 2) {
+  for (int d = threadIdx.x * 2; d < kD; d += kJoinThreads * 2) {
     float v[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kJoinWarps; ++w) {
       v[0] += f[w] * part[w][d];
       v[1] += f[w] * part[w][d + 1];
     }
@@ -665,12 +679,20 @@ template <int kD, int kNT>
 cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
   constexpr int kSmem = smem_bytes<kD, kNT>();
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  cudaError_t e = cudaFuncSetAttribute(decode_kernel<kD, kNT>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const cudaError_t e = cudaFuncSetAttribute(decode_kernel<kD, kNT>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
-  decode_kernel<kD, kNT><<<grid, kThreads, kSmem, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, decode_kernel<kD, kNT>, p);
 }
 
 template <int kD>
@@ -687,7 +709,7 @@ cudaError_t launch_join(const Params& p, int tile_rows, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), (unsigned)(most < tile_rows ? most : tile_rows),
                      p.a.cache.kv_heads);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -731,7 +753,11 @@ cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stre
   p.part_o = a.workspace;
   p.part_ml = a.workspace ? a.workspace + part_rows(a, pl) * a.cache.head_size : nullptr;
   const cudaError_t e = launch_cut(p, pl.prompt, stream);
-  return e != cudaSuccess ? e : launch_cut(p, pl.decode, stream);
+  if (e != cudaSuccess) return e;
+  // Single tokens do not depend on the prompts: their kernel may start while the
+  // last prompt tiles run.
+  p.beside = pl.prompt.rows && pl.prompt.splits == 1;
+  return launch_cut(p, pl.decode, stream);
 }
 
 }  // namespace kv
