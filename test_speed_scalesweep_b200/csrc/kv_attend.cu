@@ -513,18 +513,18 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
   if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the splits of one row, always in the same order: warp w takes splits w,
-// w + 4, ..., then the warps' results are joined.  A programmatic dependent of
-// the kernel that wrote them.
-constexpr int kJoinWarps = 4, kJoinThreads = kJoinWarps * 32;
-template <int kD>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int tile_rows) {
+// Joins the splits of a row, always in the same order: of the row's kPerRow
+// warps, warp w takes splits w, w + kPerRow, ..., then the warps' results are
+// joined.  One warp is enough for few splits (64 sequences, 6 splits: 96 us with
+// four warps per row, 93 with one), four for many.  A programmatic dependent of
+// the kernel that wrote the splits.
+template <int kD, int kPerRow>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile_rows) {
   constexpr int kPer = kD / 32;  // elements of a lane
   const AttendArgs& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int head = blockIdx.z, seq = blockIdx.x / p.tiles, r = blockIdx.y;
-  __shared__ float part[kJoinWarps][kD];
-  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
+  const int warp = (threadIdx.x >> 5) % kPerRow, lane = threadIdx.x & 31;
+  const int head = blockIdx.z, seq = blockIdx.x / p.tiles;
+  const int r = blockIdx.y * (kWarps / kPerRow) + (threadIdx.x >> 5) / kPerRow;
   // Everything that does not read the other grid's results comes before the
   // wait; CTAs without a row wait too, so that this grid does not end first.
   Tile tile;
@@ -541,56 +541,92 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const Params p, int 
   const float* po = p.part_o + out_row * kD + lane * kPer;
   const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  float mm = -INFINITY;
-  for (int s = warp + lane * kJoinWarps; s < splits; s += 32 * kJoinWarps) mm = fmaxf(mm, ml[s * step].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
-  float sum = 0.0f, acc[kPer];
+  // one pass with a running maximum, kBatch splits' loads in flight
+  constexpr int kBatch = 4;
+  float mm = -INFINITY, sum = 0.0f, acc[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) acc[j] = 0.0f;
-#pragma unroll 4
-  for (int s = warp; s < splits; s += kJoinWarps) {
-    const float2 x = ml[s * step];
-    float v[kPer];
+#pragma unroll 1
+  for (int first = warp; first < splits; first += kPerRow * kBatch) {
+    float2 x[kBatch];
+    float v[kBatch][kPer];
+    float top = mm;
 #pragma unroll
-    for (int j = 0; j < kPer / 2; ++j)
-      *reinterpret_cast<float2*>(v + 2 * j) = *reinterpret_cast<const float2*>(po + s * step * kD + 2 * j);
-    const float f = mm == -INFINITY ? 0.0f : ex2(x.x - mm);
-    sum += f * x.y;
+    for (int b = 0; b < kBatch; ++b) {
+      const int s = first + b * kPerRow;
+      x[b] = make_float2(-INFINITY, 0.0f);
+      if (s < splits) {
+        x[b] = ml[s * step];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) acc[j] += f * v[j];
-  }
+        for (int j = 0; j < kPer / 2; ++j)
+          *reinterpret_cast<float2*>(v[b] + 2 * j) =
+              *reinterpret_cast<const float2*>(po + s * step * kD + 2 * j);
+      } else {
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = acc[j];
-  if (lane == 0) {
-    part_m[warp] = mm;
-    part_l[warp] = sum;
-  }
-  __syncthreads();
-  float all = part_m[0];
-#pragma unroll
-  for (int w = 1; w < kJoinWarps; ++w) all = fmaxf(all, part_m[w]);
-  float f[kJoinWarps], total = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    f[w] = all == -INFINITY ? 0.0f : ex2(part_m[w] - all);
-    total += f[w] * part_l[w];
-  }
-  const float inv = all == -INFINITY ? 0.0f : inv_mult / total;
-  uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
-  for (int d = threadIdx.x * 2; d < kD; d += kJoinThreads * 2) {
-    float v[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      v[0] += f[w] * part[w][d];
-      v[1] += f[w] * part[w][d + 1];
+        for (int j = 0; j < kPer; ++j) v[b][j] = 0.0f;
+      }
     }
-    v[0] *= inv;
-    v[1] *= inv;
-    store16(dst + d, v, a.dtype);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) top = fmaxf(top, x[b].x);
+    if (top == -INFINITY) continue;  // no key so far
+    const float keep = ex2(mm - top);
+    mm = top;
+    sum *= keep;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) acc[j] *= keep;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const float f = ex2(x[b].x - mm);
+      sum += f * x[b].y;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) acc[j] += f * v[b][j];
+    }
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[out_row] = all == -INFINITY ? -INFINITY : (all - kShift + log2f(total)) * kLn2;
+  uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
+  if constexpr (kPerRow == 1) {
+    const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;  // a row that sees no key is zero
+#pragma unroll
+    for (int j = 0; j < kPer; j += 2) {
+      const float v[2] = {acc[j] * inv, acc[j + 1] * inv};
+      store16(dst + lane * kPer + j, v, a.dtype);
+    }
+    if (lane == 0 && a.lse)
+      a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+  } else {
+    static_assert(kPerRow == kWarps, "the CTA's row");
+    __shared__ float part[kWarps][kD];
+    __shared__ float part_m[kWarps], part_l[kWarps];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = acc[j];
+    if (lane == 0) {
+      part_m[warp] = mm;
+      part_l[warp] = sum;
+    }
+    __syncthreads();
+    float all = part_m[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) all = fmaxf(all, part_m[w]);
+    float f[kWarps], total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      f[w] = all == -INFINITY ? 0.0f : ex2(part_m[w] - all);
+      total += f[w] * part_l[w];
+    }
+    const float inv = all == -INFINITY ? 0.0f : inv_mult / total;
+    for (int d = threadIdx.x * 2; d < kD; d += kThreads * 2) {
+      float v[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        v[0] += f[w] * part[w][d];
+        v[1] += f[w] * part[w][d + 1];
+      }
+      v[0] *= inv;
+      v[1] *= inv;
+      store16(dst + d, v, a.dtype);
+    }
+    if (threadIdx.x == 0 && a.lse)
+      a.lse[out_row] = all == -INFINITY ? -INFINITY : (all - kShift + log2f(total)) * kLn2;
+  }
 }
 
 int log2i(int v) {
@@ -705,18 +741,21 @@ cudaError_t launch_rows(const Params& p, int rows, cudaStream_t stream) {
 
 template <int kD>
 cudaError_t launch_join(const Params& p, int tile_rows, cudaStream_t stream) {
-  const int64_t most = (int64_t)p.a.max_query_len * p.group;  // rows of a sequence
+  const int64_t longest = (int64_t)p.a.max_query_len * p.group;  // rows of a sequence
+  const unsigned rows = (unsigned)(longest < tile_rows ? longest : tile_rows);
+  const bool few = p.splits <= 8;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), (unsigned)(most < tile_rows ? most : tile_rows),
+  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), few ? (rows + kWarps - 1) / kWarps : rows,
                      p.a.cache.kv_heads);
-  cfg.blockDim = dim3(kJoinThreads);
+  cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, join_kernel<kD>, p, tile_rows);
+  return few ? cudaLaunchKernelEx(&cfg, join_kernel<kD, 1>, p, tile_rows)
+             : cudaLaunchKernelEx(&cfg, join_kernel<kD, kWarps>, p, tile_rows);
 }
 
 cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
