@@ -341,7 +341,7 @@ typedef struct {
  * else (2i, 2i + 1); elements past rotary_dim (a multiple of 16) are left.
  * query_out receives the rotated query (it may be query); key and value are
  * only read.  A position outside the table gives a query of NaN and writes no
- * row.  query_out must not overlap key or value.
+ * row.  query_out is query itself, or overlaps none of the inputs.
  * The bytes equal ssw_scalesweep_mse_nvfp4_quant_out's on the rotated keys,
  * rounded to their type, and the values.
  */
@@ -463,8 +463,9 @@ int ssw_kv_pages_extend(const ssw_kv_pages* tables, int64_t n, const int32_t* se
  * free ones below: afterwards pages 0 .. L - 1 are in use. */
 int ssw_kv_pages_compact(const ssw_kv_pages* tables, const ssw_kv_pool* pool, void* workspace,
                          int64_t workspace_bytes, void* stream);
-/* Page source[i] is copied to target[i] in every layer.  Targets must be
- * distinct and no source may be a target; pairs out of range are passed over. */
+/* Page source[i] is copied to target[i] in every layer, at most num_pages
+ * pairs.  Targets must be distinct and no source may be a target; pairs out of
+ * range are passed over. */
 int ssw_kv_pages_copy(const ssw_kv_pool* pool, int64_t n, const int32_t* source,
                       const int32_t* target, void* stream);
 

@@ -9,6 +9,14 @@ Drop-in for the reference's ``bench_kernel`` modules:
 * :mod:`.ops`                                   -- torch.library ops with fake impls
 * :mod:`.sharded`                               -- row-sharded multi-GPU quantization
 
+and, for the decoder layer around it:
+
+* :mod:`.act_quant`, :mod:`.norm_quant`         -- SiLU-and-mul / RMSNorm fused into the quantizer
+* :mod:`.gemm`                                  -- block-scaled NVFP4 GEMM
+* :mod:`.kv_cache`                              -- rotary positions + scale-sweep write of an NVFP4 KV cache
+* :mod:`.kv_attention`                          -- attention over that cache
+* :mod:`.kv_pages`                              -- its pages: extend, fork, free, compact, copy
+
 All compute runs in ``libscalesweep_b200.so`` (hand-written CUDA, C ABI in
 ``include/scalesweep_b200.h``).
 """

@@ -288,6 +288,11 @@ int check_pool(const char* name, const ssw_kv_pool* p, ssw::kv::PoolArgs* out) {
   if (!p->codes || !p->scales || !aligned(p->codes, 16) || !aligned(p->scales, 16))
     return fail(SSW_ERR_INVALID_ARGUMENT, "%s: codes and scales must be 16-byte aligned, not null",
                 name);
+  // items of a copy are counted in 32 bits
+  if (p->num_pages * p->layers >
+      (int64_t)((1ll << 32) / ((p->codes_page_bytes + p->scales_page_bytes) / 8192 + 2)))
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: %lld pages in %d layers are too many", name,
+                (long long)p->num_pages, p->layers);
   out->codes = p->codes;
   out->scales = p->scales;
   out->codes_layer_stride = p->codes_layer_stride;
@@ -439,7 +444,9 @@ int ssw_kv_pages_copy(const ssw_kv_pool* pool, int64_t n, const int32_t* source,
   ssw::kv::PoolArgs c;
   int st = check_pool(name, pool, &c);
   if (st != SSW_OK) return st;
-  if (n < 0 || n >= (1ll << 31)) return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad size", name);
+  if (n < 0 || n > pool->num_pages)
+    return fail(SSW_ERR_INVALID_ARGUMENT, "%s: bad size, %lld pairs of %lld pages", name,
+                (long long)n, (long long)pool->num_pages);
   if (n == 0) return SSW_OK;
   if (!source || !target || !aligned(source, 4) || !aligned(target, 4))
     return fail(SSW_ERR_INVALID_ARGUMENT, "%s: null or misaligned page list", name);

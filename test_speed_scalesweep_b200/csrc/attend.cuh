@@ -113,11 +113,11 @@ __device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int 
   const AttendArgs& a = p.a;
   const int q0 = a.query_start[seq];
   int len = a.query_start[seq + 1] - q0;
-  if (q0 < 0 || len <= 0) return false;
-  const int kv = max(0, a.seq_lens[seq]);
-  t.offset = kv - len;
-  if (q0 >= a.tokens) return false;
+  if (q0 < 0 || len <= 0 || q0 >= a.tokens) return false;
   if (len > a.tokens - q0) len = (int)(a.tokens - q0);
+  // (the bound that max_seq_len has: key numbers and their sums stay in 32 bits)
+  const int kv = min(max(0, a.seq_lens[seq]), 1 << 30);
+  t.offset = kv - len;
   const int64_t rows64 = (int64_t)len * p.group;
   if (rows64 < p.min_rows || rows64 > p.max_rows) return false;
   const int rows = (int)rows64;

@@ -103,7 +103,8 @@ struct PoolArgs {
   int64_t codes_page_bytes, scales_page_bytes;      // multiples of 16
   int64_t num_pages;
   int32_t layers;
-  int32_t code_chunks, scale_chunks;                // filled at launch
+  int32_t code_chunks, scale_chunks;                // filled at launch, as these
+  uint32_t page_magic, page_shift, layer_magic, layer_shift;  // divisions by chunks, by layers
 };
 
 int64_t pages_workspace_words(int64_t n, int64_t pages, int64_t num_pages_for_remap);

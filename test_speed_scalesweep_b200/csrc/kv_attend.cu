@@ -653,8 +653,9 @@ Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int
   c.tiles = (int)((most + tile_rows - 1) / tile_rows);
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t tokens = (tile_rows + group - 1) / group + 1;  // that a tile's rows touch
+  // a window bounds a tile's keys from both sides in the causal order only
   int64_t span = a.max_seq_len;
-  if (a.window >= 0 && span > (int64_t)a.window + tokens + kKeys)
+  if (a.causal && a.window >= 0 && span > (int64_t)a.window + tokens + kKeys)
     span = (int64_t)a.window + tokens + kKeys;
   const int64_t units = (int64_t)a.seqs * c.tiles * a.cache.kv_heads;
   // Up to three stages per warp, a second launch costs more than the split

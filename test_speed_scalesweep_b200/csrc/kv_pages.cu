@@ -15,6 +15,8 @@
 #include <cuda_runtime.h>
 
 #include "kv.cuh"
+#include "quant.cuh"
+#include "sweep.cuh"
 
 namespace ssw {
 namespace kv {
@@ -182,13 +184,16 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(const PagesArgs a, int
   }
 }
 
-// Moves kChunk bytes of page pair k's layer: items number pairs * layers * chunks.
+// Moves kChunk bytes of page pair k's layer: items number pairs * layers *
+// chunks (below 2^32: a pool's bytes over kChunk).  Divisions by multiplication:
+// 64-bit ones took as long as the copy.
 __device__ __forceinline__ void copy_item(const PoolArgs& c, const int32_t* source,
-                                          const int32_t* target, int64_t item) {
-  const int per_page = c.code_chunks + c.scale_chunks;
-  const int64_t pair_layer = item / per_page;
+                                          const int32_t* target, uint32_t item) {
+  const uint32_t per_page = c.code_chunks + c.scale_chunks;
+  const uint32_t pair_layer = div_bpc(item, c.page_magic, c.page_shift);
   const int chunk = (int)(item - pair_layer * per_page);
-  const int pair = (int)(pair_layer / c.layers), layer = (int)(pair_layer - (int64_t)pair * c.layers);
+  const uint32_t pair = div_bpc(pair_layer, c.layer_magic, c.layer_shift);
+  const uint32_t layer = pair_layer - pair * c.layers;
   const int src = source[pair], dst = target[pair];
   if ((uint32_t)src >= (uint32_t)c.num_pages || (uint32_t)dst >= (uint32_t)c.num_pages) return;
   const bool codes = chunk < c.code_chunks;
@@ -212,7 +217,7 @@ __device__ __forceinline__ void copy_item(const PoolArgs& c, const int32_t* sour
 __device__ __forceinline__ void copy_pairs(const PoolArgs& c, const int32_t* source,
                                            const int32_t* target, int64_t pairs, int first, int step) {
   const int64_t items = pairs * c.layers * (c.code_chunks + c.scale_chunks);
-  for (int64_t i = first; i < items; i += step) copy_item(c, source, target, i);
+  for (int64_t i = first; i < items; i += step) copy_item(c, source, target, (uint32_t)i);
 }
 
 // CTAs 0 .. n - 1 write the children's rows, the others copy.
@@ -281,6 +286,9 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, i
   launch_dependents();
   const PagesWork w = work_of(ws, a.n, most_pages);
   const int page_mask = (1 << a.page_shift) - 1;
+  __shared__ unsigned long long asked;  // in 64 bits: the scan's 32 could wrap
+  if (threadIdx.x == 0) asked = 0;
+  __syncthreads();
   int bad = 0, longer = 0;
   int64_t tokens = 0;
   // claim every sequence (a length becomes ~length): none may be named twice
@@ -303,6 +311,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, i
         }
       }
       w.len[i] = len;
+      if (more) atomicAdd(&asked, (unsigned long long)more);
     }
     int total;
     const int at = block_scan(more, &total);
@@ -310,7 +319,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, i
     tokens += total;
   }
   if (threadIdx.x == 0) w.first[a.n] = (int)min(tokens, (int64_t)0x7FFFFFFF);
-  if (tokens != total_tokens) bad = 1;
+  __syncthreads();
+  if (asked != (unsigned long long)total_tokens) bad = 1;
   bad = __syncthreads_or(bad);
   longer = __syncthreads_or(longer);
   // pages each request needs, in order
@@ -451,6 +461,8 @@ cudaError_t launch_after_plan(void (*kernel)(Params...), unsigned grid, cudaStre
 PoolArgs with_chunks(PoolArgs c) {
   c.code_chunks = (int)((c.codes_page_bytes + kChunk - 1) / kChunk);
   c.scale_chunks = (int)((c.scales_page_bytes + kChunk - 1) / kChunk);
+  make_divider((uint32_t)(c.code_chunks + c.scale_chunks), &c.page_magic, &c.page_shift);
+  make_divider((uint32_t)c.layers, &c.layer_magic, &c.layer_shift);
   return c;
 }
 

@@ -112,7 +112,7 @@ def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
     pairs element i with i + rotary_dim / 2, otherwise 2i with 2i + 1.
 
     Returns the rotated query: ``query_out`` if given (``query`` itself rotates
-    in place), else a new contiguous tensor.  ``key`` and ``value`` are only
+    in place, any other overlaps no input), else a new contiguous tensor.  ``key`` and ``value`` are only
     read.  Rows whose slot is negative or past the last page are padding: not
     stored.  Slots must be distinct.  A position outside the table gives NaN in
     the query, and that token is not stored."""

@@ -110,10 +110,12 @@ class Batch:
                     # floats are exact; the tensor cores may cut instead of round) of what its terms
                     # could add up to, which moves a weight and the weights' sum by as much each.
                     # A weight is rounded to f16: 2^-11, or 2^-34 of the largest where it is tiny.
-                    # The result is rounded once to its type.
+                    # The result is rounded once to its type: half a step, which for a subnormal of
+                    # the type is half its smallest one.
                     reach = scale * q[:, j].abs().amax(1, keepdim=True) * k0.abs().sum(1).amax()
                     logit_off = self.d * 2.0 ** -23 * abs(reach) + 2.0 ** -20
-                    tol = (torch.finfo(self.dtype).eps / 2 * want.abs()
+                    f = torch.finfo(self.dtype)
+                    tol = (f.eps / 2 * want.abs().clamp(min=f.smallest_normal)
                            + (2.0 ** -11 + 2 * logit_off) * weight + n * 2.0 ** -34 * v0.abs().amax())
                     off = (got[:, j] - want).abs()
                     bad = ~(off <= tol + 1e-300)
@@ -172,6 +174,15 @@ def test_without_causal_order_and_own_scale(attn, lens):
     b = Batch(lens, 4, 2, 64, 32, "f16", seed=5)
     b.check(b.call(attn, causal=False, softmax_scale=0.3), causal=False, scale=0.3)
     b.check(b.call(attn, softmax_scale=-0.2), scale=-0.2)
+    b.check(b.call(attn, softmax_scale=0.0), scale=0.0)
+
+
+@pytest.mark.parametrize("lens", [[(2592, 394), (9, 1)], [(1536, 1), (724, 4), (5000, 2)]])
+@pytest.mark.parametrize("window", [3, 211])
+def test_window_without_causal_order(attn, lens, window):
+    # such a query sees every key from window positions before it to the last one
+    b = Batch(lens, 8, 2, 64, 16, "bf16", seed=window)
+    b.check(b.call(attn, causal=False, window=window), causal=False, window=window)
 
 
 @pytest.mark.parametrize("m", [1, 140])

@@ -190,6 +190,7 @@ def test_refused_requests_change_nothing(pages):
             ("index", lambda: t.extend(i32([-1]), i32([1]), 1)),
             ("index", lambda: t.extend(i32([2]), i32([-3]), 0)),
             ("index", lambda: t.extend(i32([2]), i32([3]), 5)),
+            ("index", lambda: t.extend(i32([0, 1, 2]), i32([1 << 29, 1 << 29, 1 << 29]), 1 << 29)),
             ("not enough", lambda: t.extend(i32([2, 3]), i32([48, 48]), 96)),
             ("index", lambda: t.fork(i32([0]), i32([1]))),
             ("index", lambda: t.fork(i32([0, 0]), i32([2, 2]))),
