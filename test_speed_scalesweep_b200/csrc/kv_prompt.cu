@@ -246,65 +246,84 @@ __device__ __forceinline__ T* shfl_pointer(T* p, int from) {
       __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(p), from));
 }
 
-// The warp's 32 rows of Q as f16, scaled as in decode_kernel, into rows r0 ..
-// r0 + 31 of the swizzled tile.  Asynchronous copies bring them, neighbouring
-// lanes neighbouring parts of a row; then each thread turns its own row over in
-// place.  Short loops: this code runs once per CTA, mostly from a cold
-// instruction cache.
+// The warp's 32 rows of Q, as they are, into rows r0 .. r0 + 31 of the swizzled
+// tile: asynchronous copies, neighbouring lanes taking neighbouring parts of a
+// row; zeros for a row that is not there.
 template <int kD>
-__device__ __forceinline__ void load_queries(const Params& p, Row& w, uint32_t tile, int r0) {
+__device__ __forceinline__ void copy_queries(const Params& p, const Row& w, uint32_t tile, int r0) {
   constexpr int kLanes = kD / 8;     // lanes of a row
   constexpr int kPer = 32 / kLanes;  // rows of a warp's copy
-  const AttendArgs& a = p.a;
   const int lane = threadIdx.x & 31, part = lane % kLanes;
   const uint16_t* const mine = w.live ? w.src : nullptr;
 #pragma unroll 2
   for (int i = lane / kLanes; i < 32; i += kPer) {
     const uint16_t* src = shfl_pointer(mine, i);
-    const uint32_t bytes = src ? 16 : 0;  // zeros for a row that is not there
+    const uint32_t bytes = src ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                      tile + tile_offset(r0 + i, part)),
-                 "l"((src ? src : a.q.p) + part * 8), "r"(bytes)
+                 "l"((src ? src : p.a.q.p) + part * 8), "r"(bytes)
                  : "memory");
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncwarp();
+}
+
+// A row of 16-byte chunks of bf16 pairs times `down` as f16, in place; the
+// largest magnitude in each half of the result, as bf16 bits.
+template <int kD>
+__device__ __forceinline__ uint32_t convert_row(uint32_t tile, int r, float down) {
+  uint32_t big = 0;
+#pragma unroll 4
+  for (int j = 0; j < kD / 8; ++j) {
+    uint32_t x[4];
+    const uint32_t at = tile + tile_offset(r, j);
+    ld_shared16(at, x);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      big = __vmaxu2(big, x[c] & 0x7FFF7FFFu);
+      x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
+                     __uint_as_float(x[c] & 0xFFFF0000u) * down);
+    }
+    st_shared16(at, x[0], x[1], x[2], x[3]);
+  }
+  return big;
+}
+
+// The warp's 32 rows of Q as f16 into the swizzled tile; w.scale.  Short loops:
+// this code runs once per CTA, mostly from a cold instruction cache.
+//
+// A bf16 row whose largest magnitude lies in [2^-6, 2^15) is converted as it is:
+// no overflow, and what f16 rounds off its small elements is below 2^-19 of the
+// largest.  Other rows are fetched again and scaled by a power of two, as in
+// decode_kernel.
+template <int kD>
+__device__ __forceinline__ void load_queries(const Params& p, Row& w, uint32_t tile, int r0) {
+  const AttendArgs& a = p.a;
+  const int r = r0 + (threadIdx.x & 31);
+  copy_queries<kD>(p, w, tile, r0);
   const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
-  const bool flip = signed_log2 < 0.0f;  // the maximum is taken before scaling
+  const float sign = signed_log2 < 0.0f ? -1.0f : 1.0f;  // the maximum is taken before scaling
   float scale = fabsf(signed_log2);
   if (a.dtype == kDTypeBF16) {
-    uint32_t big = 0;
-#pragma unroll 4
-    for (int j = 0; j < kD / 8; ++j) {
-      uint32_t x[4];
-      ld_shared16(tile + tile_offset(r0 + lane, j), x);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        big = max(big, max((x[c] << 16) & 0x7FFFFFFFu, x[c] & 0x7FFF0000u));
+    const uint32_t big = convert_row<kD>(tile, r, sign);
+    const uint32_t top = max(big & 0xFFFFu, big >> 16);
+    const int e = (int)(top >> 7);  // exponent; zero, subnormal and non-finite rows stay as they are
+    const bool resize = (e >= 1 && e < 121) || (e > 141 && e <= 253);
+    if (__any_sync(0xFFFFFFFFu, resize)) {
+      __syncwarp();
+      copy_queries<kD>(p, w, tile, r0);
+      float down = sign;
+      if (resize) {
+        down *= __uint_as_float((uint32_t)(254 - e) << 23);
+        scale *= __uint_as_float((uint32_t)e << 23);
+      }
+      convert_row<kD>(tile, r, down);
     }
-    const int e = (int)(big >> 23);
-    float down = 1.0f;
-    if (e >= 1 && e <= 253) {
-      down = __uint_as_float((uint32_t)(254 - e) << 23);
-      scale *= __uint_as_float((uint32_t)e << 23);
-    }
-    if (flip) down = -down;
-#pragma unroll 4
-    for (int j = 0; j < kD / 8; ++j) {
-      uint32_t x[4];
-      const uint32_t at = tile + tile_offset(r0 + lane, j);
-      ld_shared16(at, x);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        x[c] = pack_h2(__uint_as_float(x[c] << 16) * down,
-                       __uint_as_float(x[c] & 0xFFFF0000u) * down);
-      st_shared16(at, x[0], x[1], x[2], x[3]);
-    }
-  } else if (flip) {
+  } else if (sign < 0.0f) {
 #pragma unroll 1
     for (int j = 0; j < kD / 8; ++j) {
       uint32_t x[4];
-      const uint32_t at = tile + tile_offset(r0 + lane, j);
+      const uint32_t at = tile + tile_offset(r, j);
       ld_shared16(at, x);
       st_shared16(at, x[0] ^ 0x80008000u, x[1] ^ 0x80008000u, x[2] ^ 0x80008000u,
                   x[3] ^ 0x80008000u);
