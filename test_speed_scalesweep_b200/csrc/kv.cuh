@@ -15,6 +15,35 @@
 namespace ssw {
 namespace kv {
 
+// Every kernel of the cache's operators is launched as a programmatic dependent
+// of what precedes it on the stream, so that a chain of short kernels does not
+// pay each launch in full.  Its first step is to wait for that grid, in all
+// CTAs (a grid never ends before its predecessor, and what precedes the
+// predecessor is done as well); only then may its own successor be set up,
+// which before its wait reads nothing that its predecessor writes.
+__device__ __forceinline__ void wait_for_predecessor() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void let_successor_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem,
+                             cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 struct Cache {
   uint8_t* codes;
   uint8_t* scales;

@@ -506,11 +506,13 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
 template <int kD, int kNT>
 __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
     decode_kernel(const Params p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+  // Beside a prompt kernel, which this grid does not read from and which has
+  // waited for everything before: it only ends after that one, so that what
+  // follows finds both done.
+  if (!p.beside) wait_for_predecessor();
+  let_successor_start();
   decode_tile<kD, kNT>(p);
-  // Beside a prompt kernel, which this grid does not read from: it ends after
-  // that one all the same, so that what follows finds both done.
-  if (p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.beside) wait_for_predecessor();
 }
 
 // Joins the splits of a row, always in the same order: of the row's kPerRow
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   // wait; CTAs without a row wait too, so that this grid does not end first.
   Tile tile;
   if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    wait_for_predecessor();
     return;
   }
   const int splits = used_splits(p, tile);
@@ -540,7 +542,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
   const float* po = p.part_o + out_row * kD + lane * kPer;
   const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_predecessor();
+  let_successor_start();
   // one pass with a running maximum, kBatch splits' loads in flight
   constexpr int kBatch = 4;
   float mm = -INFINITY, sum = 0.0f, acc[kPer];
@@ -716,20 +719,18 @@ template <int kD, int kNT>
 cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
   constexpr int kSmem = smem_bytes<kD, kNT>();
   static_assert(kSmem <= 227 * 1024, "shared memory");
-  const cudaError_t e = cudaFuncSetAttribute(decode_kernel<kD, kNT>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  // One sequence is cut for three CTAs per SM.  A grid set up while its
+  // predecessor still holds some SMs would put four on others and wait for
+  // those (131072 keys: 54 us against 46), so with long splits it asks for a
+  // third of the shared memory.
+  constexpr int kThird = 60 * 1024;
+  const int bytes = p.a.seqs == 1 && p.chunk >= 1024 && kSmem < kThird ? kThird : kSmem;
+  const cudaError_t e = cudaFuncSetAttribute(
+      decode_kernel<kD, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.beside ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, decode_kernel<kD, kNT>, p);
+  return launch_dependent(
+      decode_kernel<kD, kNT>,
+      dim3((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads), kThreads, bytes, stream, p);
 }
 
 template <int kD>
@@ -745,18 +746,10 @@ cudaError_t launch_join(const Params& p, int tile_rows, cudaStream_t stream) {
   const int64_t longest = (int64_t)p.a.max_query_len * p.group;  // rows of a sequence
   const unsigned rows = (unsigned)(longest < tile_rows ? longest : tile_rows);
   const bool few = p.splits <= 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.a.seqs * p.tiles), few ? (rows + kWarps - 1) / kWarps : rows,
-                     p.a.cache.kv_heads);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return few ? cudaLaunchKernelEx(&cfg, join_kernel<kD, 1>, p, tile_rows)
-             : cudaLaunchKernelEx(&cfg, join_kernel<kD, kWarps>, p, tile_rows);
+  const dim3 grid((unsigned)(p.a.seqs * p.tiles), few ? (rows + kWarps - 1) / kWarps : rows,
+                  p.a.cache.kv_heads);
+  return launch_dependent(few ? join_kernel<kD, 1> : join_kernel<kD, kWarps>, grid, kThreads, 0,
+                          stream, p, tile_rows);
 }
 
 cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {

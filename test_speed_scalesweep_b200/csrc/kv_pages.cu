@@ -26,15 +26,6 @@ constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kChunk = kCopyThreads * 2 * 16;  // bytes that a CTA moves per item
 
-// The wide kernel of a call is a programmatic dependent of its plan: it is set
-// up while the plan runs and waits for the plan's writes.
-__device__ __forceinline__ void launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void wait_for_plan() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // Exclusive scan over the CTA (1024 threads); *total gets the sum.
 __device__ __forceinline__ int block_scan(int v, int* total) {
   __shared__ int sums[32];
@@ -117,7 +108,8 @@ __device__ __host__ __forceinline__ PagesWork work_of(int32_t* w, int64_t n, int
 
 // ---- fork: the full pages are shared, a part-filled last page is copied
 __global__ void __launch_bounds__(kPlanThreads) fork_plan(const PagesArgs a, int32_t* ws) {
-  launch_dependents();
+  wait_for_predecessor();
+  let_successor_start();
   const PagesWork w = work_of(ws, a.n, a.n);
   const int page_mask = (1 << a.page_shift) - 1;
   int bad = 0, need = 0;
@@ -224,7 +216,8 @@ __device__ __forceinline__ void copy_pairs(const PoolArgs& c, const int32_t* sou
 __global__ void __launch_bounds__(kCopyThreads) fork_apply(const PagesArgs a, const PoolArgs c,
                                                            int32_t* ws) {
   const PagesWork w = work_of(ws, a.n, a.n);
-  wait_for_plan();
+  wait_for_predecessor();
+  let_successor_start();
   if (w.head[1] == 0) return;
   const int i = blockIdx.x;
   if (i >= a.n) {
@@ -250,6 +243,8 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply(const PagesArgs a, co
 
 // ---- free: one CTA per sequence; a sequence named twice is freed once
 __global__ void __launch_bounds__(kCopyThreads) free_kernel(const PagesArgs a) {
+  wait_for_predecessor();
+  let_successor_start();
   __shared__ int old;
   const int s = a.seqs[blockIdx.x];
   if ((uint32_t)s >= (uint32_t)a.max_seqs) {
@@ -283,7 +278,8 @@ __device__ __forceinline__ int last_at_most(const int32_t* starts, int n, int k)
 // ---- extend: pages for new tokens, and their slots
 __global__ void __launch_bounds__(kPlanThreads) extend_plan(const PagesArgs a, int64_t total_tokens,
                                                             int64_t most_pages, int32_t* ws) {
-  launch_dependents();
+  wait_for_predecessor();
+  let_successor_start();
   const PagesWork w = work_of(ws, a.n, most_pages);
   const int page_mask = (1 << a.page_shift) - 1;
   __shared__ unsigned long long asked;  // in 64 bits: the scan's 32 could wrap
@@ -365,7 +361,8 @@ __global__ void __launch_bounds__(kCopyThreads) extend_slots(const PagesArgs a, 
                                                              int64_t* slots) {
   const PagesWork w = work_of(ws, a.n, most_pages);
   const int64_t t = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x;
-  wait_for_plan();
+  wait_for_predecessor();
+  let_successor_start();
   if (t >= total_tokens) return;
   if (w.head[1] == 0) {
     slots[t] = -1;
@@ -379,7 +376,8 @@ __global__ void __launch_bounds__(kCopyThreads) extend_slots(const PagesArgs a, 
 
 // ---- compact: the live pages above the live count move into the holes below it
 __global__ void __launch_bounds__(kPlanThreads) compact_plan(const PagesArgs a, int32_t* ws) {
-  launch_dependents();
+  wait_for_predecessor();
+  let_successor_start();
   const PagesWork w = work_of(ws, 0, a.num_pages);
   int live = 0;
   for (int p = threadIdx.x; p < a.num_pages; p += kPlanThreads) live += a.refcount[p] != 0;
@@ -422,7 +420,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(const PagesArgs a, 
 __global__ void __launch_bounds__(kCopyThreads) compact_apply(const PagesArgs a, const PoolArgs c,
                                                               int32_t* ws) {
   const PagesWork w = work_of(ws, 0, a.num_pages);
-  wait_for_plan();
+  wait_for_predecessor();
+  let_successor_start();
   const int pairs = w.head[0];
   if (pairs == 0) return;
   copy_pairs(c, w.source, w.target, pairs, blockIdx.x, gridDim.x);
@@ -440,22 +439,9 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply(const PagesArgs a,
 
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const PoolArgs c, const int32_t* source,
                                                             const int32_t* target, int64_t pairs) {
+  wait_for_predecessor();
+  let_successor_start();
   copy_pairs(c, source, target, pairs, blockIdx.x, gridDim.x);
-}
-
-template <typename... Params, typename... Args>
-cudaError_t launch_after_plan(void (*kernel)(Params...), unsigned grid, cudaStream_t stream,
-                              Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kCopyThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 PoolArgs with_chunks(PoolArgs c) {
@@ -481,42 +467,40 @@ int64_t pages_workspace_words(int64_t n, int64_t pages, int64_t num_pages_for_re
 cudaError_t launch_fork(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, int device_sms,
                         cudaStream_t stream) {
   const PoolArgs c = with_chunks(pool);
-  fork_plan<<<1, kPlanThreads, 0, stream>>>(a, ws);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_dependent(fork_plan, dim3(1), kPlanThreads, 0, stream, a, ws);
   if (e != cudaSuccess) return e;
-  return launch_after_plan(fork_apply, a.n + copy_grid(c, a.n, device_sms), stream, a, c, ws);
+  return launch_dependent(fork_apply, dim3(a.n + copy_grid(c, a.n, device_sms)), kCopyThreads, 0,
+                          stream, a, c, ws);
 }
 
 cudaError_t launch_free(const PagesArgs& a, cudaStream_t stream) {
-  free_kernel<<<a.n, kCopyThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_dependent(free_kernel, dim3(a.n), kCopyThreads, 0, stream, a);
 }
 
 cudaError_t launch_extend(const PagesArgs& a, int64_t total_tokens, int64_t most_pages,
                           int64_t* slots, int32_t* ws, cudaStream_t stream) {
-  extend_plan<<<1, kPlanThreads, 0, stream>>>(a, total_tokens, most_pages, ws);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_dependent(extend_plan, dim3(1), kPlanThreads, 0, stream, a,
+                                         total_tokens, most_pages, ws);
   if (e != cudaSuccess || total_tokens == 0) return e;
-  return launch_after_plan(extend_slots,
-                           (unsigned)((total_tokens + kCopyThreads - 1) / kCopyThreads), stream, a,
-                           total_tokens, most_pages, ws, slots);
+  return launch_dependent(extend_slots,
+                          dim3((unsigned)((total_tokens + kCopyThreads - 1) / kCopyThreads)),
+                          kCopyThreads, 0, stream, a, total_tokens, most_pages, ws, slots);
 }
 
 cudaError_t launch_compact(const PagesArgs& a, const PoolArgs& pool, int32_t* ws, int device_sms,
                            cudaStream_t stream) {
   const PoolArgs c = with_chunks(pool);
-  compact_plan<<<1, kPlanThreads, 0, stream>>>(a, ws);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_dependent(compact_plan, dim3(1), kPlanThreads, 0, stream, a, ws);
   if (e != cudaSuccess) return e;
-  return launch_after_plan(compact_apply, copy_grid(c, a.num_pages / 2 + 1, device_sms), stream, a,
-                           c, ws);
+  return launch_dependent(compact_apply, dim3(copy_grid(c, a.num_pages / 2 + 1, device_sms)),
+                          kCopyThreads, 0, stream, a, c, ws);
 }
 
 cudaError_t launch_copy(const PoolArgs& pool, const int32_t* source, const int32_t* target,
                         int64_t pairs, int device_sms, cudaStream_t stream) {
   const PoolArgs c = with_chunks(pool);
-  copy_kernel<<<copy_grid(c, pairs, device_sms), kCopyThreads, 0, stream>>>(c, source, target, pairs);
-  return cudaGetLastError();
+  return launch_dependent(copy_kernel, dim3(copy_grid(c, pairs, device_sms)), kCopyThreads, 0, stream,
+                          c, source, target, pairs);
 }
 
 }  // namespace kv

@@ -495,7 +495,8 @@ template <int kD>
 __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   using S = PromptShape<kD>;
   extern __shared__ uint8_t smem_raw[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+  wait_for_predecessor();
+  let_successor_start();
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
@@ -687,7 +688,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
   constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kD >> 3) << 17) | (8u << 24);
   constexpr int kBarK = kBarSlot, kBarV = kBarSlot + 1;
   extern __shared__ uint8_t smem_raw[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may be set up
+  wait_for_predecessor();
+  let_successor_start();
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int seq = blockIdx.x / p.tiles, head = blockIdx.z, split = blockIdx.y;
@@ -845,8 +847,7 @@ cudaError_t launch_wide(const Params& p, cudaStream_t stream) {
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
-  prompt_wide_kernel<<<grid, kPThreads, kSmem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(prompt_wide_kernel, grid, kPThreads, kSmem, stream, p);
 }
 
 template <int kD>
@@ -857,8 +858,7 @@ cudaError_t launch_d(const Params& p, cudaStream_t stream) {
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   const dim3 grid((unsigned)(p.a.seqs * p.tiles), p.splits, p.a.cache.kv_heads);
-  prompt_kernel<kD><<<grid, kPThreads, kSmem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(prompt_kernel<kD>, grid, kPThreads, kSmem, stream, p);
 }
 
 }  // namespace

@@ -283,6 +283,8 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const KernelArgs g) 
   const uint32_t before = (uint32_t)((uint64_t)blockIdx.x * g.q_ctas / total);
   const uint32_t after = (uint32_t)(((uint64_t)blockIdx.x + 1) * g.q_ctas / total);
   if (after != before) {
+    wait_for_predecessor();
+    let_successor_start();
     rotate_query_unit<kDType, kNeox>(g, before);
     return;
   }
@@ -302,6 +304,8 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(const KernelArgs g) 
     tabw[c] = ScaleEntry{inv, mul_rn(s, s)};
   }
   __syncthreads();
+  wait_for_predecessor();
+  let_successor_start();
   quantize_units<kDType, kNeox, kLanes>(g, blockIdx.x - before, tab, tabw);
 }
 
@@ -314,6 +318,8 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherArgs p, ui
                                                           uint32_t per_token, uint32_t magic,
                                                           uint32_t shift, int d16_shift,
                                                           int page_shift) {
+  wait_for_predecessor();
+  let_successor_start();
   const uint64_t u64 = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
   if (u64 >= units) return;
   const uint32_t u = (uint32_t)u64;
@@ -361,12 +367,9 @@ int log2i(int v) {
 }
 
 template <int kDType, bool kNeox>
-void launch_lanes(const KernelArgs& g, int lanes, cudaStream_t stream) {
-  const unsigned grid = g.kv_ctas + g.q_ctas;
-  if (lanes == 4)
-    write_kernel<kDType, kNeox, 4><<<grid, kThreads, 0, stream>>>(g);
-  else
-    write_kernel<kDType, kNeox, 1><<<grid, kThreads, 0, stream>>>(g);
+cudaError_t launch_lanes(const KernelArgs& g, int lanes, cudaStream_t stream) {
+  return launch_dependent(lanes == 4 ? write_kernel<kDType, kNeox, 4> : write_kernel<kDType, kNeox, 1>,
+                          dim3(g.kv_ctas + g.q_ctas), kThreads, 0, stream, g);
 }
 
 }  // namespace
@@ -390,14 +393,11 @@ cudaError_t launch_write(const WriteArgs& a, int device_sms, cudaStream_t stream
   const uint64_t cap = (uint64_t)device_sms * 16;
   g.kv_ctas = (uint32_t)(want < cap ? want : cap);
   g.q_ctas = (uint32_t)(((uint64_t)g.q_units + kThreads - 1) / kThreads);
-  if (a.dtype == kDTypeBF16) {
-    if (a.neox) launch_lanes<kDTypeBF16, true>(g, lanes, stream);
-    else launch_lanes<kDTypeBF16, false>(g, lanes, stream);
-  } else {
-    if (a.neox) launch_lanes<kDTypeF16, true>(g, lanes, stream);
-    else launch_lanes<kDTypeF16, false>(g, lanes, stream);
-  }
-  return cudaGetLastError();
+  if (a.dtype == kDTypeBF16)
+    return a.neox ? launch_lanes<kDTypeBF16, true>(g, lanes, stream)
+                  : launch_lanes<kDTypeBF16, false>(g, lanes, stream);
+  return a.neox ? launch_lanes<kDTypeF16, true>(g, lanes, stream)
+                : launch_lanes<kDTypeF16, false>(g, lanes, stream);
 }
 
 cudaError_t launch_gather(const GatherArgs& a, int device_sms, cudaStream_t stream) {
@@ -408,13 +408,10 @@ cudaError_t launch_gather(const GatherArgs& a, int device_sms, cudaStream_t stre
   uint32_t magic, shift;
   make_divider(per_token, &magic, &shift);
   const unsigned grid = (unsigned)(((uint64_t)units + kThreads - 1) / kThreads);
-  if (a.dtype == kDTypeBF16)
-    gather_kernel<kDTypeBF16><<<grid, kThreads, 0, stream>>>(a, units, per_token, magic, shift,
-                                                            log2i((int)d16), log2i(a.cache.page_size));
-  else
-    gather_kernel<kDTypeF16><<<grid, kThreads, 0, stream>>>(a, units, per_token, magic, shift,
-                                                           log2i((int)d16), log2i(a.cache.page_size));
-  return cudaGetLastError();
+  return launch_dependent(
+      a.dtype == kDTypeBF16 ? gather_kernel<kDTypeBF16> : gather_kernel<kDTypeF16>, dim3(grid),
+      kThreads, 0, stream, a, units, per_token, magic, shift, log2i((int)d16),
+      log2i(a.cache.page_size));
 }
 
 }  // namespace kv
