@@ -59,6 +59,7 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
     ``original_max_position_embeddings``) or ``yarn`` (``factor``,
     ``original_max_position_embeddings``, optionally ``beta_fast``,
     ``beta_slow`` and ``attention_factor``, which multiplies both tables).
+    Keys that would change the frequencies in another way are refused.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
@@ -79,6 +80,9 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
         freq = torch.where(wave > original / low, freq / factor,
                            torch.where(wave < original / high, freq, between))
     elif kind == "yarn":
+        if scaling.get("mscale") or scaling.get("mscale_all_dim") or not scaling.get("truncate", True):
+            raise ValueError("yarn: mscale, mscale_all_dim and truncate=False are not supported; "
+                             "give attention_factor")
         factor, original = float(scaling["factor"]), float(scaling["original_max_position_embeddings"])
 
         def dim_of(turns):  # the pair that turns this often over the original length
@@ -112,8 +116,8 @@ def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
     pairs element i with i + rotary_dim / 2, otherwise 2i with 2i + 1.
 
     Returns the rotated query: ``query_out`` if given (``query`` itself rotates
-    in place, any other overlaps no input), else a new contiguous tensor.  ``key`` and ``value`` are only
-    read.  Rows whose slot is negative or past the last page are padding: not
+    in place, any other overlaps no input), else a new contiguous tensor.
+    ``key`` and ``value`` are only read.  Rows whose slot is negative or past the last page are padding: not
     stored.  Slots must be distinct.  A position outside the table gives NaN in
     the query, and that token is not stored."""
     return _lib.kv_binding().write(query, key, value, positions, cos_sin_cache, slot_mapping,

@@ -89,6 +89,10 @@ def test_rotary_table():
         kv_cache.rotary_cos_sin_cache(9, 8, scaling={"rope_type": "spiral"}, device="cpu")
     with pytest.raises(ValueError, match="even"):
         kv_cache.rotary_cos_sin_cache(9, 7, device="cpu")
+    for extra in ({"mscale": 1.0}, {"mscale_all_dim": 0.7}, {"truncate": False}):
+        with pytest.raises(ValueError, match="attention_factor"):
+            kv_cache.rotary_cos_sin_cache(9, 8, device="cpu", scaling=dict(
+                extra, rope_type="yarn", factor=4.0, original_max_position_embeddings=64))
 
 
 @pytest.mark.parametrize("scaling", [
