@@ -508,8 +508,12 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
     decode_kernel(const Params p) {
   // Beside a prompt kernel, which this grid does not read from and which has
   // waited for everything before: it only ends after that one, so that what
-  // follows finds both done.
-  if (!p.beside) wait_for_predecessor();
+  // follows finds both done.  Without a wait of its own at the start, a fence
+  // keeps its loads from lines that the SM's cache had before.
+  if (p.beside)
+    __threadfence();
+  else
+    wait_for_predecessor();
   let_successor_start();
   decode_tile<kD, kNT>(p);
   if (p.beside) wait_for_predecessor();
@@ -724,9 +728,11 @@ cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
   // those (131072 keys: 54 us against 46), so with long splits it asks for a
   // third of the shared memory.
   constexpr int kThird = 60 * 1024;
-  const int bytes = p.a.seqs == 1 && p.chunk >= 1024 && kSmem < kThird ? kThird : kSmem;
+  constexpr int kMost = kSmem < kThird ? kThird : kSmem;
+  const int bytes = p.a.seqs == 1 && p.chunk >= 1024 ? kMost : kSmem;
+  // always the same limit: another thread may be between this and its launch
   const cudaError_t e = cudaFuncSetAttribute(
-      decode_kernel<kD, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+      decode_kernel<kD, kNT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
   if (e != cudaSuccess) return e;
   return launch_dependent(
       decode_kernel<kD, kNT>,

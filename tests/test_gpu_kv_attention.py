@@ -263,3 +263,75 @@ def test_bounds_smaller_than_the_batch_stay_in_bounds(attn, lens):
                                          max_s, out=guard.clone())
         assert bool(out[0].isfinite().all()) and bool((out[0] != 5).any())
     b.check(b.call(attn))
+
+
+@pytest.mark.parametrize("lens", [[(4096, 1)] * 3, [(2048, 300), (4096, 1), (64, 1)], [(5000, 1)]])
+def test_reads_what_the_launch_before_wrote(attn, lens):
+    """Launches overlap their predecessors' ends: inputs written just before a call, into lines that the call
+    before it has read, are the ones that it sees."""
+    b, c = Batch(lens, 8, 2, 128, 16, "bf16", seed=4), Batch(lens, 8, 2, 128, 16, "bf16", seed=6)
+    fewer = [(n - 1, q) for n, q in lens]
+    c.seq_lens.copy_(torch.tensor([n for n, _ in fewer], dtype=torch.int32))
+    inputs = [[t.clone() for t in (x.q, x.codes, x.raw, x.table, x.seq_lens, x.mult)] for x in (b, c)]
+    inputs[1][5].mul_(2)
+    mine = (b.q, b.codes, b.raw, b.table, b.seq_lens, b.mult)
+
+    def load(which):
+        for dst, src in zip(mine, inputs[which]):
+            dst.copy_(src)
+    want = []
+    for which in (0, 1):
+        load(which)
+        torch.cuda.synchronize()
+        want.append(b.call(attn))
+        torch.cuda.synchronize()
+    got = []
+    for i in range(24):
+        load(i % 2)
+        got.append(b.call(attn))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert torch.equal(out, want[i % 2]), i
+
+
+def test_two_host_threads(attn):
+    """Calls of two threads through the C interface, which holds no lock: a long sequence and a batch of short
+    ones use one kernel with different launch settings."""
+    import ctypes
+    import threading
+
+    from test_speed_scalesweep_b200 import _lib
+    lib = _lib.lib()
+    jobs = []
+    for lens in ([(60000, 1)], [(900, 1)] * 4):
+        b = Batch(lens, 8, 8, 128, 16, "bf16", seed=5)
+        want = b.call(attn)
+        out = torch.empty_like(want)
+        cache = _lib.KVCache(codes=b.codes.data_ptr(), scales=b.raw.data_ptr(), codes_page_stride=b.codes.stride(0),
+                             scales_page_stride=b.raw.stride(0), input_scale=b.mult.data_ptr(),
+                             num_pages=b.codes.shape[0], page_size=16, kv_heads=8, head_size=128)
+        args = _lib.KVAttention(block_table=b.table.data_ptr(), block_table_stride=b.table.stride(0),
+                                seq_lens=b.seq_lens.data_ptr(), query_start=b.start.data_ptr(), tokens=len(lens),
+                                seqs=len(lens), block_table_columns=b.table.shape[1], q_heads=8, max_query_len=1,
+                                max_seq_len=b.max_s, causal=1, window=-1, softmax_scale=128 ** -0.5)
+        q, o = _lib.KVHeads(b.q.data_ptr(), 8 * 128, 128), _lib.KVHeads(out.data_ptr(), 8 * 128, 128)
+        need = lib.ssw_nvfp4_paged_attention_workspace_bytes(ctypes.byref(cache), ctypes.byref(args), 0)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+        jobs.append((b, want, out, (ctypes.byref(cache), ctypes.byref(args), 0, ctypes.byref(q), ctypes.byref(o),
+                                    ws.data_ptr(), need, torch.cuda.Stream().cuda_stream), ws))
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(call):
+        for _ in range(400):
+            if lib.ssw_nvfp4_paged_attention(*call) != 0:
+                bad.append(lib.ssw_last_error())
+    threads = [threading.Thread(target=run, args=(j[3],)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad, bad[:1]
+    for _, want, out, _, _ in jobs:
+        assert torch.equal(out, want)
