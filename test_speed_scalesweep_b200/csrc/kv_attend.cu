@@ -653,8 +653,10 @@ struct Plan {
   Cut decode, prompt;
 };
 
-// `most` rows at most per sequence; `target` CTAs keep the GPU busy evenly.
-Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int64_t min_chunk) {
+// `most` rows at most per sequence.  The keys are cut so that `wave` CTAs fill
+// the GPU once, and finer, into `fine` CTAs, as far as splits stay `floor` keys.
+Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t wave, int64_t fine,
+           int64_t floor, int64_t min_chunk) {
   Cut c = {};
   c.rows = tile_rows;
   c.tiles = (int)((most + tile_rows - 1) / tile_rows);
@@ -665,17 +667,39 @@ Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t target, int
   if (a.causal && a.window >= 0 && span > (int64_t)a.window + tokens + kKeys)
     span = (int64_t)a.window + tokens + kKeys;
   const int64_t units = (int64_t)a.seqs * c.tiles * a.cache.kv_heads;
-  // Up to three stages per warp, a second launch costs more than the split
-  // saves (1 sequence of 300 keys: 8.2 us in one CTA per head, 9.2 split; of
-  // 700 keys 12.3 and 9.4).
-  const bool whole = target / units < 1 || (span <= 384 && tile_rows <= 8);
-  const int64_t splits = whole ? 1 : target / units;
-  int64_t chunk = ((span + splits - 1) / splits + 127) / 128 * 128;
+  auto chunk_for = [&](int64_t ctas) {
+    const int64_t splits = ctas / units < 1 ? 1 : ctas / units;
+    return ((span + splits - 1) / splits + 127) / 128 * 128;
+  };
+  int64_t chunk = chunk_for(wave);
+  const int64_t finer = chunk_for(fine) < floor ? floor : chunk_for(fine);
+  if (chunk > finer) chunk = finer;
+  // Two stages per warp cost less than the second launch (one sequence of 256
+  // keys: 5.8 us in one CTA per head, 6.2 split; of 300 keys 7.0 and 6.3).
+  if (span <= 256 && tile_rows <= 8) chunk = 256;
   if (chunk < min_chunk) chunk = min_chunk;
   c.chunk = (int)chunk;
   // the first key of a windowed tile is rounded down to a stage
   c.splits = (int)((span + (a.window >= 0 ? kKeys - 1 : 0) + chunk - 1) / chunk);
   return c;
+}
+
+// A start and a partial result are what a split costs, so the keys are cut into
+// one wave of CTAs: 4 per SM with 8 rows and heads up to 128, else 2 (8
+// sequences of 4096 keys: 16.2 us, cut into two waves 18.9, into six 24).
+// Sequences of several lengths are cut finer, into up to 24 CTAs per SM, so that
+// the longest do not run on alone (64 of up to 8192 keys: 89 us, 98 with 12 per
+// SM), but not below 1024 keys (16 of up to 8192: 27 us, 30 with 512) or, two
+// per SM, 2048 (16 rows, 64 of up to 8192: 78 us, 82 with 1024).  A single
+// sequence takes 3 and 2 CTAs per SM (131072 keys: 45 us, 60 with 4; with 16
+// rows 36 us, 50 with 3).
+Cut decode_cut(const AttendArgs& a, int tile_rows, int64_t most, int64_t sms) {
+  const bool four = tile_rows == 8 && a.cache.head_size <= 128;
+  if (a.seqs == 1) {
+    const int64_t wave = sms * (four ? 3 : 2);
+    return cut_of(a, tile_rows, most, wave, wave, 128, 128);
+  }
+  return cut_of(a, tile_rows, most, sms * (four ? 4 : 2), sms * 24, four ? 1024 : 2048, 128);
 }
 
 Plan plan_of(const AttendArgs& a, int device_sms) {
@@ -685,23 +709,18 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
   // 32 rows per kv head: heads of 64 198 us here, 224 on the tensor cores' own
   // memory; heads of 128 331 and 262).
   const int most = a.cache.head_size == 64 ? 32 : 16;
-  // A single sequence is cut into one wave of CTAs (1 x 131072 keys, 8 kv heads:
-  // 53 us with 3 CTAs per SM, 57 with 8, 70 with 12, each with a start and a
-  // partial result of its own).  Sequences of several lengths are cut finer, so
-  // that the longest do not run on alone (64 of up to 8192: 100 us with 24,
-  // 111 with 12, 117 with 72).
-  const int64_t target = (int64_t)device_sms * (a.seqs == 1 ? 3 : 24);
+  const int64_t sms = device_sms;
   Plan pl = {};
   if (rows <= most) {
-    pl.decode = cut_of(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, target, 128);
+    pl.decode = decode_cut(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, sms);
     pl.decode.max_rows = 0x7FFFFFFF;
     return pl;
   }
-  pl.prompt = cut_of(a, prompt_rows(a.cache.head_size), rows, device_sms, 512);
+  pl.prompt = cut_of(a, prompt_rows(a.cache.head_size), rows, sms, sms, 512, 512);
   pl.prompt.prompt = 1;
   pl.prompt.max_rows = 0x7FFFFFFF;
   if (a.seqs > 1) {  // single tokens among prompts
-    pl.decode = cut_of(a, group <= 8 ? 8 : 16, 16, target, 128);
+    pl.decode = decode_cut(a, group <= 8 ? 8 : 16, 16, sms);
     pl.decode.max_rows = pl.decode.rows;
     pl.decode.tiles = 1;
     pl.prompt.min_rows = pl.decode.rows + 1;
