@@ -654,7 +654,8 @@ struct Plan {
 };
 
 // `most` rows at most per sequence.  The keys are cut so that `wave` CTAs fill
-// the GPU once, and finer, into `fine` CTAs, as far as splits stay `floor` keys.
+// the GPU once or, where `fine` is more, into that many as far as splits keep
+// `floor` keys; never below `min_chunk`.
 Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t wave, int64_t fine,
            int64_t floor, int64_t min_chunk) {
   Cut c = {};
@@ -672,8 +673,10 @@ Cut cut_of(const AttendArgs& a, int tile_rows, int64_t most, int64_t wave, int64
     return ((span + splits - 1) / splits + 127) / 128 * 128;
   };
   int64_t chunk = chunk_for(wave);
-  const int64_t finer = chunk_for(fine) < floor ? floor : chunk_for(fine);
-  if (chunk > finer) chunk = finer;
+  if (fine > wave) {
+    const int64_t finer = chunk_for(fine) < floor ? floor : chunk_for(fine);
+    if (chunk > finer) chunk = finer;
+  }
   // Two stages per warp cost less than the second launch (one sequence of 256
   // keys: 5.8 us in one CTA per head, 6.2 split; of 300 keys 7.0 and 6.3).
   if (span <= 256 && tile_rows <= 8) chunk = 256;
@@ -697,7 +700,7 @@ Cut decode_cut(const AttendArgs& a, int tile_rows, int64_t most, int64_t sms) {
   const bool four = tile_rows == 8 && a.cache.head_size <= 128;
   if (a.seqs == 1) {
     const int64_t wave = sms * (four ? 3 : 2);
-    return cut_of(a, tile_rows, most, wave, wave, 128, 128);
+    return cut_of(a, tile_rows, most, wave, wave, 0, 128);
   }
   return cut_of(a, tile_rows, most, sms * (four ? 4 : 2), sms * 24, four ? 1024 : 2048, 128);
 }
@@ -716,7 +719,17 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
     pl.decode.max_rows = 0x7FFFFFFF;
     return pl;
   }
-  pl.prompt = cut_of(a, prompt_rows(a.cache.head_size), rows, sms, sms, 512, 512);
+  // One wave of CTAs, one per SM.  What a split costs (a launch, partial results
+  // of all its rows) pays down to 256 keys where one tile holds all rows (64
+  // queries, 2048 keys: 15.3 us, 18.1 with 512), else to 512 (512 queries, 512
+  // keys: 15.7, 20.8 with 256).  Several such sequences are cut finer, to even
+  // out their lengths (16 queries each of 4 of up to 65536 keys: 180 us, 235 in
+  // one wave), those of more rows are not (500 each of 8 of up to 4096: 184, 243
+  // with splits of 2048).
+  const int tile_rows = prompt_rows(a.cache.head_size);
+  const bool one = rows <= tile_rows;
+  pl.prompt = cut_of(a, tile_rows, rows, sms, one && a.seqs > 1 ? sms * 4 : sms, 2048,
+                     one ? 256 : 512);
   pl.prompt.prompt = 1;
   pl.prompt.max_rows = 0x7FFFFFFF;
   if (a.seqs > 1) {  // single tokens among prompts
