@@ -521,9 +521,8 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
 
 // Joins the splits of a row, always in the same order: of the row's kPerRow
 // warps, warp w takes splits w, w + kPerRow, ..., then the warps' results are
-// joined.  One warp is enough for few splits (64 sequences, 6 splits: 96 us with
-// four warps per row, 93 with one), four for many.  A programmatic dependent of
-// the kernel that wrote the splits.
+// joined.  One warp is enough for few splits (64 sequences, 6 splits: 91 us with
+// four warps per row, 89 with one), four for many.
 template <int kD, int kPerRow>
 __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile_rows) {
   constexpr int kPer = kD / 32;  // elements of a lane

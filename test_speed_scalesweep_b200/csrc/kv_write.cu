@@ -126,7 +126,8 @@ __device__ __forceinline__ void rotate_pairs4(uint4& x, const float* cs, int hal
 }
 
 // Query heads per thread: they share the position's cosines and sines (64
-// bytes for 32 bytes of a head), and their loads are in flight together.
+// bytes for 32 bytes of a head), and their loads are in flight together (8192
+// tokens of 32 + 8 heads of 128: 69.7 us with one, 61.4 with two, 59.4 with four).
 constexpr int kQHeads = 4;
 
 struct KernelArgs {

@@ -1,6 +1,6 @@
 // The scale sweep of one 16-element block, shared by every kernel that
 // quantizes: candidate errors, the window's argmin, block amax and the tables
-// of E4M3 scales they read.  Included by quant.cu and kv_write.cu.
+// of E4M3 scales they read; and division by a launch constant.
 #pragma once
 
 #include <cstdint>
