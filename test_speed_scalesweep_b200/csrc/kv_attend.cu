@@ -707,14 +707,16 @@ Cut decode_cut(const AttendArgs& a, int tile_rows, int64_t most, int64_t sms) {
 Plan plan_of(const AttendArgs& a, int device_sms) {
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t rows = (int64_t)a.max_query_len * group;
-  // Rows up to which decode_kernel is the faster one (32 sequences of 8192 keys,
-  // 32 rows per kv head: heads of 64 198 us here, 224 on the tensor cores' own
-  // memory; heads of 128 331 and 262).
-  const int most = a.cache.head_size == 64 ? 32 : 16;
+  // Rows up to which decode_kernel is the faster one (32 sequences of 8192 keys, 8
+  // kv heads, 32 rows: heads of 64 in one tile 148 us, 231 on the tensor cores'
+  // own memory; heads of 128 in two tiles of 16 239 and 271; heads of 256 so 422
+  // and 372).
+  const int most = a.cache.head_size == 256 ? 16 : 32;
   const int64_t sms = device_sms;
   Plan pl = {};
   if (rows <= most) {
-    pl.decode = decode_cut(a, rows <= 8 ? 8 : rows <= 16 ? 16 : most, rows, sms);
+    const int tile_rows = rows <= 8 ? 8 : rows <= 16 || a.cache.head_size == 128 ? 16 : 32;
+    pl.decode = decode_cut(a, tile_rows, rows, sms);
     pl.decode.max_rows = 0x7FFFFFFF;
     return pl;
   }
