@@ -370,8 +370,9 @@ int ssw_nvfp4_kv_gather(const ssw_kv_cache* cache, int dtype, int64_t tokens,
  * that a window has left behind).  Query i of a sequence has the position
  * seq_lens[b] - (its query rows) + i; causal: it sees the keys up to that
  * position; window >= 0: only those from position - window on.  A row that
- * sees no key gives zeros and a log-sum-exp of -inf.  Rows of out and lse that
- * belong to no sequence are left as they were.
+ * sees no key gives zeros and a log-sum-exp of -inf; a NaN score, or infinite
+ * ones as the softmax takes them, give NaN.  Rows of out and lse that belong to
+ * no sequence are left as they were.
  * out[r] = sum_j softmax_j(softmax_scale * q[r] . K[j]) V[j]; query head h uses
  * kv head h / (q_heads / kv_heads).  lse (may be null): float [tokens,
  * q_heads], the natural log of the sum of exp(softmax_scale * q . K).

@@ -143,6 +143,23 @@ __device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
   return min(max(1, (n + p.chunk - 1) / p.chunk), p.splits);
 }
 
+// How a row is finished.  Its sum l of weights says whether it saw a key: a key
+// that it sees adds 2^kShift or more to l by the time the maximum m is final, a
+// masked one exactly 0.  A row whose scores so far are all -inf has m = -inf; the
+// keys that it saw are counted in l, so that it is told from a row that saw
+// none, and the count is dropped (times 2^-inf) when a larger score comes.  A
+// NaN score makes l NaN and leaves m alone.
+
+// 1 / (l * multiplier); 0 for a row that saw no key, whose result is zero; NaN
+// where every score is -inf, the weights being 0 / 0.
+__device__ __forceinline__ float row_inverse(float m, float l, float inv_mult) {
+  return l == 0.0f ? 0.0f : m == -INFINITY ? NAN : inv_mult / l;
+}
+// Natural log-sum-exp: -inf for a row that saw no key (-inf + log2 0).
+__device__ __forceinline__ float row_lse(float m, float l) { return (m - kShift + log2f(l)) * kLn2; }
+// The weight of a partial result with the maximum x where the joint one is m.
+__device__ __forceinline__ float part_weight(float x, float m) { return x == m ? 1.0f : ex2(x - m); }
+
 __device__ __forceinline__ void store16(uint16_t* dst, const float* v, int dtype) {  // 2 values
   if (dtype == kDTypeBF16) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);

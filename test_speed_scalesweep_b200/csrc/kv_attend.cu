@@ -311,7 +311,7 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
     bool grow = false;
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[2] = {-INFINITY, -INFINITY}, seen[2] = {4.0f, 4.0f};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -320,8 +320,10 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
           if constexpr (masked) {
             const int key = k0 + h * 16 + key_a + 8 * (c >> 1);
             const bool here = (came >> (pieces == 2 ? h : 0)) & 1u;
-            if (!here || key >= c1 || key > hi_key[n][c & 1] || key < lo_key[n][c & 1])
+            if (!here || key >= c1 || key > hi_key[n][c & 1] || key < lo_key[n][c & 1]) {
               v = -INFINITY;
+              seen[c & 1] -= 1.0f;
+            }
           }
           s[h][n][c] = v;
           mx[c & 1] = fmaxf(mx[c & 1], v);
@@ -350,6 +352,9 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
       }
       const float m0 = m[n][0] == -INFINITY ? 0.0f : m[n][0] - kShift;
       const float m1 = m[n][1] == -INFINITY ? 0.0f : m[n][1] - kShift;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)  // keys seen whose scores are all -inf: see row_inverse
+        if (m[n][c] == -INFINITY) l[n][c] += seen[c];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float p0 = ex2(fmaf(s[h][n][0], scale[n][0], -m0));
@@ -478,7 +483,7 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
     float o[2] = {0.0f, 0.0f}, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = mm == -INFINITY ? 0.0f : ex2(x[w * kStride + kD] - mm);
+      const float f = part_weight(x[w * kStride + kD], mm);
       sum += f * x[w * kStride + kD + 1];
       o[0] += f * x[w * kStride + d];
       o[1] += f * x[w * kStride + d + 1];
@@ -487,14 +492,13 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
     const int qh = head * p.group + row % p.group;
     const int64_t out_row = (int64_t)token * a.q_heads + qh;
     if (p.splits == 1) {
-      // a row that sees no key is zero
-      const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;
+      const float inv = row_inverse(mm, sum, inv_mult);
       o[0] *= inv;
       o[1] *= inv;
       store16(a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride + d,
               o, a.dtype);
       if (d == 0 && a.lse)
-        a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+        a.lse[out_row] = row_lse(mm, sum);
     } else {
       const int64_t at_row = (int64_t)split * a.tokens * a.q_heads + out_row;
       *reinterpret_cast<float2*>(p.part_o + at_row * kD + d) = make_float2(o[0], o[1]);
@@ -574,15 +578,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) top = fmaxf(top, x[b].x);
-    if (top == -INFINITY) continue;  // no key so far
-    const float keep = ex2(mm - top);
+    const float keep = part_weight(mm, top);
     mm = top;
     sum *= keep;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) acc[j] *= keep;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const float f = ex2(x[b].x - mm);
+      const float f = part_weight(x[b].x, mm);
       sum += f * x[b].y;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) acc[j] += f * v[b][j];
@@ -590,14 +593,13 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   }
   uint16_t* dst = a.out.p + (int64_t)token * a.out.token_stride + (int64_t)qh * a.out.head_stride;
   if constexpr (kPerRow == 1) {
-    const float inv = mm == -INFINITY ? 0.0f : inv_mult / sum;  // a row that sees no key is zero
+    const float inv = row_inverse(mm, sum, inv_mult);
 #pragma unroll
     for (int j = 0; j < kPer; j += 2) {
       const float v[2] = {acc[j] * inv, acc[j + 1] * inv};
       store16(dst + lane * kPer + j, v, a.dtype);
     }
-    if (lane == 0 && a.lse)
-      a.lse[out_row] = mm == -INFINITY ? -INFINITY : (mm - kShift + log2f(sum)) * kLn2;
+    if (lane == 0 && a.lse) a.lse[out_row] = row_lse(mm, sum);
   } else {
     static_assert(kPerRow == kWarps, "the CTA's row");
     __shared__ float part[kWarps][kD];
@@ -615,10 +617,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
     float f[kWarps], total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      f[w] = all == -INFINITY ? 0.0f : ex2(part_m[w] - all);
+      f[w] = part_weight(part_m[w], all);
       total += f[w] * part_l[w];
     }
-    const float inv = all == -INFINITY ? 0.0f : inv_mult / total;
+    const float inv = row_inverse(all, total, inv_mult);
     for (int d = threadIdx.x * 2; d < kD; d += kThreads * 2) {
       float v[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -630,8 +632,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
       v[1] *= inv;
       store16(dst + d, v, a.dtype);
     }
-    if (threadIdx.x == 0 && a.lse)
-      a.lse[out_row] = all == -INFINITY ? -INFINITY : (all - kShift + log2f(total)) * kLn2;
+    if (threadIdx.x == 0 && a.lse) a.lse[out_row] = row_lse(all, total);
   }
 }
 

@@ -391,6 +391,8 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
       }
     }
   }
+  if (m == -INFINITY)  // a key seen whose score is -inf: see row_inverse
+    l += !masked || (mask[0] | mask[1] | mask[2] | mask[3]) ? 1.0f : 0.0f;
   const float ms = m == -INFINITY ? 0.0f : m - kShift;
   const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
   uint64_t sums[2] = {0, 0};
@@ -445,10 +447,10 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int 
                                              uint32_t o_addr, uint32_t stage, bool any, float m,
                                              float l) {
   const AttendArgs& a = p.a;
-  const bool seen = any && m != -INFINITY;  // a row that sees no key is zero
+  const bool seen = any && l != 0.0f;  // a row that saw no key is zero
   const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + w.out_row;
   if (p.splits == 1) {
-    const float inv = seen ? 1.0f / __ldg(a.cache.multiplier + 1) / l : 0.0f;
+    const float inv = row_inverse(m, l, 1.0f / __ldg(a.cache.multiplier + 1));
 #pragma unroll 1
     for (int c = 0; c < kD / 64; ++c) {
       uint32_t h[32];
@@ -473,7 +475,7 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int 
       }
       store_rows(stage, h, w.live ? reinterpret_cast<uint8_t*>(w.dst + 64 * c) : nullptr);
     }
-    if (w.live && a.lse) a.lse[w.out_row] = seen ? (m - kShift + log2f(l)) * kLn2 : -INFINITY;
+    if (w.live && a.lse) a.lse[w.out_row] = row_lse(m, l);
   } else {
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {

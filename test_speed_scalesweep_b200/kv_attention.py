@@ -32,7 +32,8 @@ def nvfp4_paged_attention(query: torch.Tensor, codes: torch.Tensor, scales: torc
     ``causal``: a query sees the keys up to its own position, its sequence's
     queries being the last of its keys.  ``window``: only those at most
     ``window`` positions before it.  ``softmax_scale`` defaults to D ** -0.5.
-    A row that sees no key gives zeros (log-sum-exp -inf).
+    A row that sees no key gives zeros (log-sum-exp -inf); NaN or an infinity in
+    a query row that sees one gives NaN, in that row alone.
 
     Returns ``out`` [T, Hq, D] of the query's type (rows of no sequence are left
     as they were; without ``out`` a new tensor, those rows undefined), with
