@@ -19,8 +19,12 @@ namespace kv {
 // of what precedes it on the stream, so that a chain of short kernels does not
 // pay each launch in full.  Its first step is to wait for that grid, in all
 // CTAs (a grid never ends before its predecessor, and what precedes the
-// predecessor is done as well); only then may its own successor be set up,
-// which before its wait reads nothing that its predecessor writes.
+// predecessor is done as well) before it reads anything; only then may its own
+// successor be set up.  Inputs are read by plain loads: a non-coherent one asks
+// that its memory stays unwritten while the grid lives, and the grid lives
+// before its predecessor has written.  What reads inputs without a wait
+// (join_kernel's tile, decode_kernel beside a prompt kernel) has a predecessor
+// that waited for their writers and writes none of them, and fences first.
 __device__ __forceinline__ void wait_for_predecessor() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

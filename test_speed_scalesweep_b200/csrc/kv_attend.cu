@@ -118,20 +118,21 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
                             (scales_part ? S::kKCodes : 0) + my_piece * copy_bytes;
   const int copy_key = c0 + warp * kKeys + my_piece * piece;  // of stage 0
   const int copy_end = copies ? min((int64_t)tile.end, (int64_t)c0 + p.chunk) : 0;
-  auto page_of = [&](int i) -> int {  // the page of this lane's piece of stage i, or -1
+  // The table's entry for this lane's piece of stage i, or -1; looked at only
+  // where it is used, a stage later.
+  auto page_of = [&](int i) -> int {
     const int k = copy_key + i * (kWarps * kKeys);
-    if (k >= copy_end) return -1;
-    const int pg = __ldg(table + (k >> p.page_shift));
-    return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
+    return k < copy_end ? table[k >> p.page_shift] : -1;
   };
   // Starts stage i's copies into ring slot `slot`; which lanes' pieces exist.
   auto issue = [&](int i, int slot, int pg) -> uint32_t {
     const uint32_t bar = bars + 8 * slot;
-    const uint32_t live = __ballot_sync(0xFFFFFFFFu, pg >= 0);
+    const bool there = (uint32_t)pg < (uint32_t)a.cache.num_pages;
+    const uint32_t live = __ballot_sync(0xFFFFFFFFu, there);
     if (lane == 0)
       mbar_expect_tx(bar, (uint32_t)(__popc(live) / 4) * (uint32_t)(S::kStage / kKeys * piece));
     __syncwarp();
-    if (pg >= 0) {
+    if (there) {
       const int k = copy_key + i * (kWarps * kKeys);
       bulk_load(copy_dst + slot * S::kStage,
                 copy_src + pg * page_stride + (k & (page_rows - 1)) * row_bytes, copy_bytes, bar);
@@ -153,7 +154,7 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
   int lo_key[kNT][2], hi_key[kNT][2];
   float acc[kNT][kD / 16][4], m[kNT][2], l[kNT][2];
   // the sign of the scale goes into Q, so that a larger score is a larger weight
-  const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  const float signed_log2 = a.softmax_scale * kLog2e / *a.cache.multiplier;
   const float to_log2 = fabsf(signed_log2);
   const bool flip = signed_log2 < 0.0f;
 #pragma unroll
@@ -471,7 +472,7 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
       }
     }
   __syncthreads();
-  const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
+  const float inv_mult = 1.0f / a.cache.multiplier[1];
   const float* all = reinterpret_cast<const float*>(smem);
   constexpr int kStride = kRows * (kD + 2);
   for (int at = threadIdx.x; at < tile.rows * (kD / 2); at += kThreads) {
@@ -512,12 +513,15 @@ __global__ void __launch_bounds__(kThreads, kNT == 1 && kD <= 128 ? 4 : 1)
     decode_kernel(const Params p) {
   // Beside a prompt kernel, which this grid does not read from and which has
   // waited for everything before: it only ends after that one, so that what
-  // follows finds both done.  Without a wait of its own at the start, a fence
-  // keeps its loads from lines that the SM's cache had before.
-  if (p.beside)
+  // follows finds both done.  Without a wait of its own at the start, fences
+  // keep its loads from lines that the SM's cache had before, and order its bulk
+  // copies behind what was written by plain stores.
+  if (p.beside) {
     __threadfence();
-  else
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+  } else {
     wait_for_predecessor();
+  }
   let_successor_start();
   decode_tile<kD, kNT>(p);
   if (p.beside) wait_for_predecessor();
@@ -535,7 +539,11 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const int head = blockIdx.z, seq = blockIdx.x / p.tiles;
   const int r = blockIdx.y * (kWarps / kPerRow) + (threadIdx.x >> 5) / kPerRow;
   // Everything that does not read the other grid's results comes before the
-  // wait; CTAs without a row wait too, so that this grid does not end first.
+  // wait (behind it, 64 sequences took 95 us against 94): the other grid has
+  // let this one start after waiting for what wrote the inputs, and writes none
+  // of them itself; the fence keeps these loads from lines that the SM's cache
+  // had before.  CTAs without a row wait too, so that this grid does not end first.
+  __threadfence();
   Tile tile;
   if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) {
     wait_for_predecessor();
@@ -548,7 +556,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const int64_t step = a.tokens * a.q_heads;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
   const float* po = p.part_o + out_row * kD + lane * kPer;
-  const float inv_mult = 1.0f / __ldg(a.cache.multiplier + 1);
+  const float inv_mult = 1.0f / a.cache.multiplier[1];
   wait_for_predecessor();
   let_successor_start();
   // one pass with a running maximum, kBatch splits' loads in flight

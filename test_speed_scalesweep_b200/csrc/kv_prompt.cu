@@ -182,13 +182,13 @@ __device__ __forceinline__ void load_row(RowRegs<kD>& r, const uint8_t* codes,
   if (there) {
 #pragma unroll
     for (int j = 0; j < kD / 32; ++j)
-      *reinterpret_cast<uint4*>(&r.codes[4 * j]) = __ldg(reinterpret_cast<const uint4*>(codes) + j);
+      *reinterpret_cast<uint4*>(&r.codes[4 * j]) = reinterpret_cast<const uint4*>(codes)[j];
     if constexpr (kD == 64) {
-      r.scales[0] = __ldg(reinterpret_cast<const uint32_t*>(scales));
+      r.scales[0] = *reinterpret_cast<const uint32_t*>(scales);
     } else if constexpr (kD == 128) {
-      *reinterpret_cast<uint2*>(r.scales) = __ldg(reinterpret_cast<const uint2*>(scales));
+      *reinterpret_cast<uint2*>(r.scales) = *reinterpret_cast<const uint2*>(scales);
     } else {
-      *reinterpret_cast<uint4*>(r.scales) = __ldg(reinterpret_cast<const uint4*>(scales));
+      *reinterpret_cast<uint4*>(r.scales) = *reinterpret_cast<const uint4*>(scales);
     }
   } else {  // what lies behind the last key may hold anything, NaN scales too
 #pragma unroll
@@ -301,7 +301,7 @@ __device__ __forceinline__ void load_queries(const Params& p, Row& w, uint32_t t
   const AttendArgs& a = p.a;
   const int r = r0 + (threadIdx.x & 31);
   copy_queries<kD>(p, w, tile, r0);
-  const float signed_log2 = a.softmax_scale * kLog2e / __ldg(a.cache.multiplier);
+  const float signed_log2 = a.softmax_scale * kLog2e / *a.cache.multiplier;
   const float sign = signed_log2 < 0.0f ? -1.0f : 1.0f;  // the maximum is taken before scaling
   float scale = fabsf(signed_log2);
   if (a.dtype == kDTypeBF16) {
@@ -450,7 +450,7 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int 
   const bool seen = any && l != 0.0f;  // a row that saw no key is zero
   const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + w.out_row;
   if (p.splits == 1) {
-    const float inv = row_inverse(m, l, 1.0f / __ldg(a.cache.multiplier + 1));
+    const float inv = row_inverse(m, l, 1.0f / a.cache.multiplier[1]);
 #pragma unroll 1
     for (int c = 0; c < kD / 64; ++c) {
       uint32_t h[32];
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     auto page_of = [&](int j) -> int {
       const int key = c0 + j * kBlock + i;
       if (key >= c1 || key < tile.beg) return -1;
-      const int pg = __ldg(table + (key >> p.page_shift));
+      const int pg = table[key >> p.page_shift];
       return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
     };
     auto fetch = [&](RowRegs<kD>& r, int j, int pg, int value) {
@@ -772,7 +772,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     auto page_of = [&](int j) -> int {
       const int key = c0 + j * kBlock + i;
       if (key >= c1 || key < tile.beg) return -1;
-      const int pg = __ldg(table + (key >> p.page_shift));
+      const int pg = table[key >> p.page_shift];
       return (uint32_t)pg < (uint32_t)a.cache.num_pages ? pg : -1;
     };
     auto fetch = [&](RowRegs<kD>& r, int j, int pg) {

@@ -27,7 +27,7 @@ namespace {
 constexpr int kThreads = 256;  // the shared tables rely on it
 
 __device__ __forceinline__ uint4 ld16(const uint16_t* p) {
-  return __ldg(reinterpret_cast<const uint4*>(p));
+  return *reinterpret_cast<const uint4*>(p);
 }
 
 template <int kDType>
@@ -60,10 +60,10 @@ __device__ __forceinline__ void rotate_half8(uint4& own, const uint4& other, con
   uint32_t* o = reinterpret_cast<uint32_t*>(&own);
   const uint32_t* t = reinterpret_cast<const uint32_t*>(&other);
   float c[8], s[8];
-  *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs));
-  *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(cs) + 1);
-  *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(cs + half));
-  *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(cs + half) + 1);
+  *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs);
+  *reinterpret_cast<float4*>(c + 4) = reinterpret_cast<const float4*>(cs)[1];
+  *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(cs + half);
+  *reinterpret_cast<float4*>(s + 4) = reinterpret_cast<const float4*>(cs + half)[1];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float a0, a1, b0, b1;
@@ -114,8 +114,8 @@ template <int kDType>
 __device__ __forceinline__ void rotate_pairs4(uint4& x, const float* cs, int half) {
   uint32_t* w = reinterpret_cast<uint32_t*>(&x);
   float c[4], s[4];
-  *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(cs));
-  *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(cs + half));
+  *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs);
+  *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(cs + half);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float a, b;
@@ -146,7 +146,7 @@ __device__ __forceinline__ void quantize_units(const KernelArgs& g, uint32_t cta
   const WriteArgs& p = g.a;
   const int half = p.rotary_dim >> 1;
   const uint32_t sub = threadIdx.x % kLanes;
-  const float mult_k = __ldg(p.cache.multiplier), mult_v = __ldg(p.cache.multiplier + 1);
+  const float mult_k = *p.cache.multiplier, mult_v = p.cache.multiplier[1];
   // Whole warps stay in the loop: the lanes of a shared unit exchange winners.
   constexpr uint32_t kPerCta = kThreads / kLanes;
   const uint32_t warp_first = (threadIdx.x & ~31u) / kLanes;
@@ -161,8 +161,8 @@ __device__ __forceinline__ void quantize_units(const KernelArgs& g, uint32_t cta
     r >>= g.d16_shift;
     const bool is_value = r >= (uint32_t)p.cache.kv_heads;
     const uint32_t head = is_value ? r - p.cache.kv_heads : r;
-    const int64_t slot = __ldg(p.slots + token);
-    const int64_t pos = __ldg(p.positions + token);
+    const int64_t slot = p.slots[token];
+    const int64_t pos = p.positions[token];
     const bool write = in && slot >= 0 && (slot >> g.page_shift) < p.cache.num_pages &&
                        (uint64_t)pos < (uint64_t)p.max_position;
     uint4 x[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
@@ -244,7 +244,7 @@ __device__ __forceinline__ void rotate_query_unit(const KernelArgs& g, uint32_t 
       p.q.p + (int64_t)token * p.q.token_stride + (int64_t)head * p.q.head_stride;
   uint16_t* dst = p.q_out.p + (int64_t)token * p.q_out.token_stride +
                   (int64_t)head * p.q_out.head_stride;
-  const int64_t pos = __ldg(p.positions + token);
+  const int64_t pos = p.positions[token];
   const bool known = (uint64_t)pos < (uint64_t)p.max_position;
   // plain loads: the output may be the query itself
   uint4 x[kQHeads], y[kQHeads];
@@ -261,8 +261,8 @@ __device__ __forceinline__ void rotate_query_unit(const KernelArgs& g, uint32_t 
     const float* cs = p.cos_sin + pos * p.rotary_dim + (kNeox ? o1 : o1 / 2);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      *reinterpret_cast<float4*>(c + 4 * j) = __ldg(reinterpret_cast<const float4*>(cs) + j);
-      *reinterpret_cast<float4*>(s + 4 * j) = __ldg(reinterpret_cast<const float4*>(cs + half) + j);
+      *reinterpret_cast<float4*>(c + 4 * j) = reinterpret_cast<const float4*>(cs)[j];
+      *reinterpret_cast<float4*>(s + 4 * j) = reinterpret_cast<const float4*>(cs + half)[j];
     }
   }
 #pragma unroll
@@ -330,20 +330,20 @@ __global__ void __launch_bounds__(kThreads) gather_kernel(const GatherArgs p, ui
   const uint32_t side_head = r >> d16_shift;
   const bool is_value = side_head >= (uint32_t)p.cache.kv_heads;
   const uint32_t head = is_value ? side_head - p.cache.kv_heads : side_head;
-  const int64_t slot = __ldg(p.slots + token);
+  const int64_t slot = p.slots[token];
   uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (slot >= 0 && (slot >> page_shift) < p.cache.num_pages) {
     const int64_t page = slot >> page_shift;
     const int64_t row = ((int64_t)side_head << page_shift) + (slot & ((1 << page_shift) - 1));
     const int64_t at = (row << d16_shift) + block;
-    const uint2 c = __ldg(reinterpret_cast<const uint2*>(
-        p.cache.codes + page * p.cache.codes_page_stride + at * 8));
+    const uint2 c = *reinterpret_cast<const uint2*>(
+        p.cache.codes + page * p.cache.codes_page_stride + at * 8);
     uint32_t s2;  // the scale as f16, exact
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
         : "=r"(s2)
-        : "h"((uint16_t)__ldg(p.cache.scales + page * p.cache.scales_page_stride + at)));
+        : "h"((uint16_t)p.cache.scales[page * p.cache.scales_page_stride + at]));
     const float s = __fdiv_rn(__low2float(*reinterpret_cast<const __half2*>(&s2)),
-                              __ldg(p.cache.multiplier + (is_value ? 1 : 0)));
+                              p.cache.multiplier[is_value ? 1 : 0]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       uint32_t h[4];
