@@ -29,8 +29,11 @@ struct Params {
   int beside;      // 1: decode_kernel launched while a prompt kernel may still run
   int chunk;       // keys of a split, a multiple of 128
   int page_shift;
-  float* part_o;   // [split][row of q and head][head_size]
-  float* part_ml;  // [split][row of q and head][2]
+  // Partial results: [split][part_rows][head_size], and [..][2] of maximum and sum
+  float* part_o;
+  float* part_ml;
+  int64_t part_rows;
+  int part_seq_rows;  // rows kept per sequence and kv head; 0: a row per token and query head
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -134,6 +137,15 @@ __device__ __forceinline__ bool tile_of(const Params& p, int seq, int tile, int 
   t.all_beg = a.window >= 0 ? max(0, hi - a.window) : 0;
   t.end = max(t.end, 0);
   return true;
+}
+
+// Where split `split` of row `row` of a sequence (row `out_row` of the batch) keeps its partial result.
+__device__ __forceinline__ int64_t part_row(const Params& p, int split, int seq, int head, int row,
+                                            int64_t out_row) {
+  return split * p.part_rows +
+         (p.part_seq_rows
+              ? ((int64_t)seq * p.a.cache.kv_heads + head) * p.part_seq_rows + row
+              : out_row);
 }
 
 // Splits of a tile that hold keys (at least one, which then writes zeros).  A

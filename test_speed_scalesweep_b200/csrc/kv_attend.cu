@@ -501,7 +501,7 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
       if (d == 0 && a.lse)
         a.lse[out_row] = row_lse(mm, sum);
     } else {
-      const int64_t at_row = (int64_t)split * a.tokens * a.q_heads + out_row;
+      const int64_t at_row = part_row(p, split, seq, head, row, out_row);
       *reinterpret_cast<float2*>(p.part_o + at_row * kD + d) = make_float2(o[0], o[1]);
       if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at_row * 2) = make_float2(mm, sum);
     }
@@ -553,9 +553,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const int row = tile.row0 + r, token = tile.first_token + row / p.group;
   const int qh = head * p.group + row % p.group;
   const int64_t out_row = (int64_t)token * a.q_heads + qh;
-  const int64_t step = a.tokens * a.q_heads;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + out_row;
-  const float* po = p.part_o + out_row * kD + lane * kPer;
+  const int64_t step = p.part_rows, first_part = part_row(p, 0, seq, head, row, out_row);
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + first_part;
+  const float* po = p.part_o + first_part * kD + lane * kPer;
   const float inv_mult = 1.0f / a.cache.multiplier[1];
   wait_for_predecessor();
   let_successor_start();
@@ -751,15 +751,23 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
   return pl;
 }
 
-int most_splits(const Plan& pl) {
-  const int a = pl.decode.rows ? pl.decode.splits : 1, b = pl.prompt.rows ? pl.prompt.splits : 1;
-  return a > b ? a : b;
+// The rows of one cut's partial results, for each of its splits: those of the
+// batch or, where that is less, as many per sequence as the cut takes (single
+// tokens among the rows of prompts; a query tensor padded far past its rows).
+// The two cuts' kernels follow each other where both are split, so they share
+// the memory.
+struct Parts {
+  int64_t rows;  // of a split; 0: not split
+  int seq_rows;  // Params::part_seq_rows
+};
+Parts parts_of(const AttendArgs& a, const Cut& c) {
+  if (c.rows == 0 || c.splits == 1) return {0, 0};
+  const int64_t all = a.tokens * a.q_heads, seq_rows = (int64_t)c.tiles * c.rows;
+  const int64_t some = (int64_t)a.seqs * a.cache.kv_heads * seq_rows;
+  return some < all ? Parts{some, (int)seq_rows} : Parts{all, 0};
 }
 
-int64_t part_rows(const AttendArgs& a, const Plan& pl) {
-  const int splits = most_splits(pl);
-  return splits > 1 ? (int64_t)splits * a.tokens * a.q_heads : 0;
-}
+int64_t part_rows(const AttendArgs& a, const Cut& c) { return parts_of(a, c).rows * c.splits; }
 
 template <int kD, int kNT>
 cudaError_t launch_decode(const Params& p, cudaStream_t stream) {
@@ -807,6 +815,11 @@ cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
   p.chunk = c.chunk;
   p.min_rows = c.min_rows;
   p.max_rows = c.max_rows;
+  const Parts parts = parts_of(p.a, c);
+  p.part_rows = parts.rows;
+  p.part_seq_rows = parts.seq_rows;
+  p.part_o = p.a.workspace;
+  p.part_ml = p.a.workspace + parts.rows * c.splits * p.a.cache.head_size;
   const int d = p.a.cache.head_size;
   cudaError_t e = c.prompt   ? launch_prompt(p, stream)
                   : d == 64  ? launch_rows<64>(p, c.rows, stream)
@@ -821,7 +834,9 @@ cudaError_t launch_cut(Params p, const Cut& c, cudaStream_t stream) {
 }  // namespace
 
 int64_t attend_workspace_bytes(const AttendArgs& a, int device_sms) {
-  return part_rows(a, plan_of(a, device_sms)) * (a.cache.head_size + 2) * (int64_t)sizeof(float);
+  const Plan pl = plan_of(a, device_sms);
+  const int64_t x = part_rows(a, pl.decode), y = part_rows(a, pl.prompt);
+  return (x > y ? x : y) * (a.cache.head_size + 2) * (int64_t)sizeof(float);
 }
 
 cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stream) {
@@ -831,8 +846,6 @@ cudaError_t launch_attend(const AttendArgs& a, int device_sms, cudaStream_t stre
   if (a.window > (1 << 30)) p.a.window = 1 << 30;  // positions stay below it
   p.group = a.q_heads / a.cache.kv_heads;
   p.page_shift = log2i(a.cache.page_size);
-  p.part_o = a.workspace;
-  p.part_ml = a.workspace ? a.workspace + part_rows(a, pl) * a.cache.head_size : nullptr;
   const cudaError_t e = launch_cut(p, pl.prompt, stream);
   if (e != cudaSuccess) return e;
   // Single tokens do not depend on the prompts: their kernel may start while the

@@ -443,12 +443,11 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[3
 // The rows' results from O (kD columns at o_addr): out, or a split's partial.
 // `stage`: 4 KB of shared memory of the warp's own.
 template <int kD>
-__device__ __forceinline__ void store_result(const Params& p, const Row& w, int split,
+__device__ __forceinline__ void store_result(const Params& p, const Row& w, int64_t part_row,
                                              uint32_t o_addr, uint32_t stage, bool any, float m,
                                              float l) {
   const AttendArgs& a = p.a;
   const bool seen = any && l != 0.0f;  // a row that saw no key is zero
-  const int64_t part_row = (int64_t)split * a.tokens * a.q_heads + w.out_row;
   if (p.splits == 1) {
     const float inv = row_inverse(m, l, 1.0f / a.cache.multiplier[1]);
 #pragma unroll 1
@@ -659,8 +658,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
     // this half's MMAs are done with its Q, which becomes the staging area
-    store_result<kD>(p, w, split, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
-                     work && blocks > 0, m, l);
+    store_result<kD>(p, w, part_row(p, split, seq, head, tile.row0 + half * 128 + r, w.out_row), o_addr,
+                     q_tile + half * S::kTile + (warp & 3) * 4096, work && blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
@@ -832,7 +831,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     if (blocks > 1 && ok) ok = mbar_wait(o_done, (blocks - 2) & 1);
     if (blocks > 0 && ok) ok = mbar_wait(o_done, (blocks - 1) & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    store_result<kD>(p, w, split, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
+    store_result<kD>(p, w, part_row(p, split, seq, head, tile.row0 + r, w.out_row), tmem + lanes + kO,
+                     q_tile + warp * 4096, blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
