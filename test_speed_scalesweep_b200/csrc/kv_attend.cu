@@ -742,10 +742,10 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
                      one ? 256 : 512);
   pl.prompt.prompt = 1;
   pl.prompt.max_rows = 0x7FFFFFFF;
-  if (a.seqs > 1) {  // single tokens among prompts
-    pl.decode = decode_cut(a, group <= 8 ? 8 : 16, 16, sms);
-    pl.decode.max_rows = pl.decode.rows;
-    pl.decode.tiles = 1;
+  if (a.seqs > 1) {  // single tokens among prompts (how many is not known here: as if all were)
+    const int few = group <= 8 ? 8 : 16;
+    pl.decode = decode_cut(a, few, few, sms);
+    pl.decode.max_rows = few;
     pl.prompt.min_rows = pl.decode.rows + 1;
   }
   return pl;

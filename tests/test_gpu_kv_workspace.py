@@ -45,6 +45,17 @@ def test_prompts_beside_single_tokens(attn, hq, hkv, d, prompt, singles, keys): 
     assert got <= min(most, 128 * MIB), (got, most)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (24, 6, 64), (8, 1, 256), (32, 2, 128)])
+@pytest.mark.parametrize("seqs,keys", [(2, 131072), (5, 30000), (24, 8192)])
+def test_single_tokens_beside_prompts_are_cut_as_alone(attn, hq, hkv, d, seqs, keys):  # noqa: F811
+    tile = 8 if hq // hkv <= 8 else 16
+    prompt = 128  # one tile or two of each sequence, whose own partial results are smaller
+    mixed, alone = need(hq, hkv, d, seqs, seqs * prompt, prompt, keys), need(hq, hkv, d, seqs, seqs, 1, keys)
+    splits, rest = divmod(alone, seqs * hq * (d + 2) * 4)
+    assert rest == 0 and splits > 1
+    assert mixed >= splits * seqs * hkv * tile * (d + 2) * 4
+
+
 @pytest.mark.parametrize("hq,hkv,d,seqs,max_q", [(32, 8, 128, 1, 1), (8, 8, 64, 3, 2), (16, 2, 128, 2, 100)])
 def test_a_padded_query_tensor_costs_nothing(attn, hq, hkv, d, seqs, max_q):  # noqa: F811
     tight = need(hq, hkv, d, seqs, seqs * max_q, max_q, 65536)
