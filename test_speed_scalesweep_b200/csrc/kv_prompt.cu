@@ -678,7 +678,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
 // 12: MMAs.
 struct WideControl {
   uint64_t s_full[2];  // scores are in buffer 0 / 1 (and K's tile is free)
-  uint64_t o_done;     // a P V has completed (and V's tile is free)
+  uint64_t o_done;     // a P V before the last has completed (and V's tile is free)
+  uint64_t o_last;     // the last one has
 };
 static_assert(sizeof(WideControl) <= sizeof(uint64_t) * 6, "fits in front of Control's masks");
 
@@ -707,11 +708,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
   Control* ctl = reinterpret_cast<Control*>(smem_raw + (smem + 3 * kTile - smem_u32(smem_raw)));
   WideControl* wide = reinterpret_cast<WideControl*>(ctl);  // over empty[] and s_full[]
   const uint32_t s_full[2] = {smem_u32(&wide->s_full[0]), smem_u32(&wide->s_full[1])};
-  const uint32_t o_done = smem_u32(&wide->o_done);
+  const uint32_t o_done = smem_u32(&wide->o_done), o_last = smem_u32(&wide->o_last);
   if (threadIdx.x == 0) {
     mbar_init(s_full[0], 1);
     mbar_init(s_full[1], 1);
     mbar_init(o_done, 1);
+    mbar_init(o_last, 1);
     for (int i = 0; i < kMaskRing; ++i) mbar_init(smem_u32(&ctl->mask_full[i]), 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
           for (int i = 0; i < kBlock / 16; ++i)
             mma_ts(tmem + kO, tmem + 128 * (j & 1) + 8 * i, smem_desc(v_tile + 2048 * i, 16384, 1024),
                    kIdescPV, (j | i) != 0);
-          mma_commit(o_done);
+          mma_commit(j + 1 < blocks ? o_done : o_last);
         }
       }
       __syncwarp();
@@ -826,10 +828,11 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
       // be two ahead, the scores after the next being issued behind this P V.
       bar_arrive(kBarP + (j & 1), 128 + 32);
     }
-    // The last scores only tell that the P V two blocks before has completed: a
-    // parity wait may not skip the one between.
-    if (blocks > 1 && ok) ok = mbar_wait(o_done, (blocks - 2) & 1);
-    if (blocks > 0 && ok) ok = mbar_wait(o_done, (blocks - 1) & 1);
+    // The last P V has a barrier of its own.  On o_done a warp would have to wait
+    // for the one before it first, since a parity wait may not skip a phase, and
+    // the last could complete before that wait looks: the phase that it waits for
+    // would be gone, and the wait run out.
+    if (blocks > 0 && ok) ok = mbar_wait(o_last, 0);
     asm volatile("tcgen05.fence::after_thread_sync;");
     store_result<kD>(p, w, part_row(p, split, seq, head, tile.row0 + r, w.out_row), tmem + lanes + kO,
                      q_tile + warp * 4096, blocks > 0, m, l);
