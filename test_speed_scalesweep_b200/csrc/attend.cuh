@@ -157,10 +157,10 @@ __device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
 
 // How a row is finished.  Its sum l of weights says whether it saw a key: a key
 // that it sees adds 2^kShift or more to l by the time the maximum m is final, a
-// masked one exactly 0.  A row whose scores so far are all -inf has m = -inf; the
-// keys that it saw are counted in l, so that it is told from a row that saw
-// none, and the count is dropped (times 2^-inf) when a larger score comes.  A
-// NaN score makes l NaN and leaves m alone.
+// masked one exactly 0.  A row whose scores so far are all -inf has m = -inf and a
+// positive l (in decode_kernel the keys that it saw), so that it is told from a
+// row that saw none; that l is dropped (times 2^-inf) when a larger score comes.
+// A NaN score makes l NaN and leaves m alone.
 
 // 1 / (l * multiplier); 0 for a row that saw no key, whose result is zero; NaN
 // where every score is -inf, the weights being 0 / 0.

@@ -351,11 +351,12 @@ __device__ __forceinline__ bool block_mask(const Control* ctl, int j, int k0, co
 // Softmax of the 128 scores at s_addr: updates the row's maximum and sum,
 // rescales O (kD columns at o_addr) where the maximum has grown by more than
 // the slack, and writes P over the scores.  `before_rescale` runs before O is
-// touched.
+// touched.  `saw` becomes nonzero where the row sees a key.
 template <int kD, typename F>
 __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, bool masked,
                                               const uint32_t (&mask)[4], float scale, bool first,
-                                              float& m, float& l, F&& before_rescale) {
+                                              float& m, float& l, uint32_t& saw,
+                                              F&& before_rescale) {
   uint32_t v[128];
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -365,6 +366,9 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
 #pragma unroll
     for (int x = 0; x < 128; ++x)
       if (!((mask[x / 32] >> (x % 32)) & 1u)) v[x] = 0xFF800000u;
+    saw |= mask[0] | mask[1] | mask[2] | mask[3];
+  } else {
+    saw = 1;
   }
   float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -391,8 +395,6 @@ __device__ __forceinline__ void softmax_block(uint32_t s_addr, uint32_t o_addr, 
       }
     }
   }
-  if (m == -INFINITY)  // a key seen whose score is -inf: see row_inverse
-    l += !masked || (mask[0] | mask[1] | mask[2] | mask[3]) ? 1.0f : 0.0f;
   const float ms = m == -INFINITY ? 0.0f : m - kShift;
   const uint64_t scale2 = pack2(scale, scale), ms2 = pack2(-ms, -ms);
   uint64_t sums[2] = {0, 0};
@@ -440,10 +442,11 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[3
   __syncwarp();
 }
 
-// The rows' results from O (kD columns at o_addr): out, or a split's partial.
+// The rows' results from O (kD columns at o_addr): out, or a split's partial;
+// this thread's is row `row_in` of the tile.
 // `stage`: 4 KB of shared memory of the warp's own.
 template <int kD>
-__device__ __forceinline__ void store_result(const Params& p, const Row& w, int64_t part_row,
+__device__ __forceinline__ void store_result(const Params& p, const Row& w, int row_in,
                                              uint32_t o_addr, uint32_t stage, bool any, float m,
                                              float l) {
   const AttendArgs& a = p.a;
@@ -476,6 +479,11 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int6
     }
     if (w.live && a.lse) a.lse[w.out_row] = row_lse(m, l);
   } else {
+    // from the launch's coordinates, which are at hand here: carried through the
+    // blocks, the place costs the softmax threads registers
+    const int tile = p.tiles - 1 - blockIdx.x % p.tiles;
+    const int64_t part = part_row(p, blockIdx.y, blockIdx.x / p.tiles, blockIdx.z,
+                                  tile * prompt_rows(kD) + row_in, w.out_row);
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
       uint32_t v[32];
@@ -486,9 +494,9 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int6
 #pragma unroll
       for (int x = 0; x < 32; ++x) v[x] = seen ? v[x] : 0;
       store_rows(stage, v,
-                 w.live ? reinterpret_cast<uint8_t*>(p.part_o + part_row * kD + 32 * c) : nullptr);
+                 w.live ? reinterpret_cast<uint8_t*>(p.part_o + part * kD + 32 * c) : nullptr);
     }
-    if (w.live) *reinterpret_cast<float2*>(p.part_ml + part_row * 2) = make_float2(m, l);
+    if (w.live) *reinterpret_cast<float2*>(p.part_ml + part * 2) = make_float2(m, l);
   }
 }
 
@@ -644,6 +652,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     const uint32_t s_addr = tmem + lanes + S::kS + 128 * half;
     const uint32_t o_addr = tmem + lanes + S::kO + kD * half;
     float m = -INFINITY, l = 0.0f;
+    uint32_t saw = 0;
     const bool work = half == 0 || two;
     for (int j = 0; work && j < blocks; ++j) {
       if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
@@ -652,14 +661,15 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       if (ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), j & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
       // the P V before this S was issued before it, and has completed with it
-      softmax_block<kD>(s_addr, o_addr, masked, mask, w.scale, j == 0, m, l, [] {});
+      softmax_block<kD>(s_addr, o_addr, masked, mask, w.scale, j == 0, m, l, saw, [] {});
       bar_arrive(kBarP + half, 128 + 32);
     }
     if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
+    if (saw && l == 0.0f) l = 1.0f;  // all its scores are -inf: see row_inverse
     // this half's MMAs are done with its Q, which becomes the staging area
-    store_result<kD>(p, w, part_row(p, split, seq, head, tile.row0 + half * 128 + r, w.out_row), o_addr,
-                     q_tile + half * S::kTile + (warp & 3) * 4096, work && blocks > 0, m, l);
+    store_result<kD>(p, w, half * 128 + r, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
+                     work && blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
@@ -810,6 +820,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     bar_arrive(kBarQ, 128 + 32);
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     float m = -INFINITY, l = 0.0f;
+    uint32_t saw = 0;
     for (int j = 0; j < blocks; ++j) {
       if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
@@ -819,7 +830,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
       // these scores were issued before the last P V, which O's rescaling must
       // wait for
       softmax_block<kD>(tmem + lanes + 128 * (j & 1), tmem + lanes + kO, masked, mask, w.scale,
-                        j == 0, m, l, [&] {
+                        j == 0, m, l, saw, [&] {
                           if (ok) ok = mbar_wait(o_done, (j - 1) & 1);
                           asm volatile("tcgen05.fence::after_thread_sync;");
                         });
@@ -834,8 +845,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     // would be gone, and the wait run out.
     if (blocks > 0 && ok) ok = mbar_wait(o_last, 0);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    store_result<kD>(p, w, part_row(p, split, seq, head, tile.row0 + r, w.out_row), tmem + lanes + kO,
-                     q_tile + warp * 4096, blocks > 0, m, l);
+    if (saw && l == 0.0f) l = 1.0f;
+    store_result<kD>(p, w, r, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
   }
   if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
