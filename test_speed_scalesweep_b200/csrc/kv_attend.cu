@@ -235,10 +235,10 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
     const int k0 = c0 + (warp + i * kWarps) * kKeys;
     const int page_ahead = next_page;
     next_page = page_of(i + 1 + S::kStages);
-    if (!mbar_wait(bars + 8 * slot, phase)) {
+    if (!warp_wait(bars + 8 * slot, phase)) {
       // give up: the copies still in flight get their (bounded) time to land
       for (int j = i; j < n_stages && j < i + S::kStages; ++j)
-        mbar_wait(bars + 8 * (j % S::kStages), (j / S::kStages) & 1);
+        warp_wait(bars + 8 * (j % S::kStages), (j / S::kStages) & 1);
       ok = false;
       break;
     }

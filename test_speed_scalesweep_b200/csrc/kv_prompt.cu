@@ -23,7 +23,8 @@
 // next S has (MMAs complete in order), and the next one waits for this P.
 //
 // Every mbarrier wait is bounded; after one that gave up the roles keep their
-// barrier protocol, so no partner is left waiting, and *status is set.
+// barrier protocol, so no partner is left waiting (see bar_tell), MMAs in flight
+// are waited for, with a limit, and *status is set.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -57,8 +58,21 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
-// Named barriers: tile slots 1..4 full, P of half 0 / 1, Q loaded.
-constexpr int kBarSlot = 1, kBarP = 5, kBarQ = 7;
+// Named barriers, 16 of hardware: the tiles that K and V are dequantized into
+// are full, P is there, Q is loaded.  A warp that only tells the MMA warp arrives
+// and goes on, so it may be ahead of it by as many of its arrivals as its waits
+// for the MMAs allow.  Each kind therefore has a barrier more for every arrival
+// that may be outstanding where such a wait gives up, used in turn: from then on
+// the warp waits at its barriers too (bar_tell), and so it can never arrive twice
+// at one before the MMA warp has, which would end that barrier's phase without
+// it and leave it waiting for good.
+//   prompt_kernel: K (V) of a block waits for the MMAs that read its slot, two
+//   blocks before: the last three arrivals may be outstanding, 8 barriers for 4
+//   slots; P waits for scores issued behind the P before the last: 2 a half.
+//   prompt_wide_kernel: K and V wait for the MMAs of the block before: 2 each; P
+//   waits for scores issued behind the P before the last two: 4.
+constexpr int kBarSlot = 1, kBarP = 9, kBarQ = 13;
+constexpr int kBarWideK = 1, kBarWideV = 3, kBarWideP = 5;
 
 template <int kD>
 struct PromptShape {
@@ -77,7 +91,9 @@ struct Control {
   uint64_t s_full[2];
   uint64_t mask_full[kMaskRing];
   uint32_t mask[kMaskRing][4];  // bit i: key i of the block is there
+  uint64_t drained;             // after a wait that gave up: every MMA has completed
   uint32_t tmem;
+  uint32_t gave_up;
 };
 
 __device__ __forceinline__ void bar_sync(int id, int threads) {
@@ -85,6 +101,13 @@ __device__ __forceinline__ void bar_sync(int id, int threads) {
 }
 __device__ __forceinline__ void bar_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// The same `ok` in all of the warp.
+__device__ __forceinline__ void bar_tell(bool ok, int id, int threads) {
+  if (ok)
+    bar_arrive(id, threads);
+  else
+    bar_sync(id, threads);
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -442,6 +465,22 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[3
   __syncwarp();
 }
 
+// A wait has given up: what the caller, and the end of the CTA, go by.
+__device__ __forceinline__ void give_up(Control* ctl, int32_t* status) {
+  *reinterpret_cast<volatile uint32_t*>(&ctl->gave_up) = 1;
+  if (status) atomicCAS(status, 0, 1);
+}
+
+// The MMA warp, behind the last barrier: where a wait gave up, MMAs may still be
+// in flight, which read shared memory, write TMEM and arrive on barriers.  Waits
+// for them, with a limit as well, before TMEM is freed and the CTA ends.
+__device__ __forceinline__ void drain_after_giving_up(Control* ctl) {
+  if (*reinterpret_cast<const volatile uint32_t*>(&ctl->gave_up) == 0) return;
+  if ((threadIdx.x & 31) == 0) mma_commit(smem_u32(&ctl->drained));
+  mbar_wait(smem_u32(&ctl->drained), 0);
+  __syncwarp();
+}
+
 // The rows' results from O (kD columns at o_addr): out, or a split's partial;
 // this thread's is row `row_in` of the tile.
 // `stage`: 4 KB of shared memory of the warp's own.
@@ -528,6 +567,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&ctl->empty[i]), 1);
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctl->s_full[i]), 1);
     for (int i = 0; i < kMaskRing; ++i) mbar_init(smem_u32(&ctl->mask_full[i]), 4);
+    mbar_init(smem_u32(&ctl->drained), 1);
+    ctl->gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kWarpMma) {
@@ -568,7 +609,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       }
     };
     if (blocks > 0) {
-      bar_sync(kBarSlot, 128 + 32);
+      bar_sync(kBarSlot, 128 + 32);  // K of block j: kBarSlot + 2j mod 8, V: the next
       asm volatile("tcgen05.fence::after_thread_sync;");
       qk(0, 0);
       if (two) qk(1, 0);
@@ -578,12 +619,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       for (int j = 0; j < blocks; ++j) {
         const int v_slot = (2 * j + 1) & 3, k_slot = (2 * j + 2) & 3;
         const bool more = j + 1 < blocks;
-        bar_sync(kBarSlot + v_slot, 128 + 32);
-        if (more) bar_sync(kBarSlot + k_slot, 128 + 32);
+        bar_sync(kBarSlot + ((2 * j + 1) & 7), 128 + 32);
+        if (more) bar_sync(kBarSlot + ((2 * j + 2) & 7), 128 + 32);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (half == 1 && !two) break;
-          bar_sync(kBarP + half, 128 + 32);
+          bar_sync(kBarP + 2 * half + (j & 1), 128 + 32);
           asm volatile("tcgen05.fence::after_thread_sync;");
           pv(half, v_slot, j == 0);
           if (more)
@@ -623,21 +664,21 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       const int k_slot = (2 * j) & 3, v_slot = k_slot + 1;
       const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
       // slots are used every second block
-      if (j >= 2 && ok) ok = mbar_wait(smem_u32(&ctl->empty[k_slot]), ((j >> 1) - 1) & 1);
+      if (j >= 2 && ok) ok = warp_wait(smem_u32(&ctl->empty[k_slot]), ((j >> 1) - 1) & 1);
       if (lane == 0) {
         ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
         mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
       }
       store_row<kD>(k, ring + k_slot * S::kTile, i);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(kBarSlot + k_slot, 128 + 32);
+      bar_tell(ok, kBarSlot + ((2 * j) & 7), 128 + 32);
       pg = pg_next;
       pg_next = page_of(j + 2);
       fetch(k, j + 1, pg, 0);
-      if (j >= 2 && ok) ok = mbar_wait(smem_u32(&ctl->empty[v_slot]), ((j >> 1) - 1) & 1);
+      if (j >= 2 && ok) ok = warp_wait(smem_u32(&ctl->empty[v_slot]), ((j >> 1) - 1) & 1);
       store_row<kD>(v, ring + v_slot * S::kTile, i);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(kBarSlot + v_slot, 128 + 32);
+      bar_tell(ok, kBarSlot + ((2 * j + 1) & 7), 128 + 32);
       fetch(v, j + 1, pg, 1);
     }
   } else {
@@ -655,27 +696,28 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     uint32_t saw = 0;
     const bool work = half == 0 || two;
     for (int j = 0; work && j < blocks; ++j) {
-      if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      if (ok) ok = warp_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
       const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
-      if (ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), j & 1);
+      if (ok) ok = warp_wait(smem_u32(&ctl->s_full[half]), j & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
       // the P V before this S was issued before it, and has completed with it
       softmax_block<kD>(s_addr, o_addr, masked, mask, w.scale, j == 0, m, l, saw, [] {});
-      bar_arrive(kBarP + half, 128 + 32);
+      bar_tell(ok, kBarP + 2 * half + (j & 1), 128 + 32);
     }
-    if (work && blocks > 0 && ok) ok = mbar_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
+    if (work && blocks > 0 && ok) ok = warp_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
     if (saw && l == 0.0f) l = 1.0f;  // all its scores are -inf: see row_inverse
     // this half's MMAs are done with its Q, which becomes the staging area
     store_result<kD>(p, w, half * 128 + r, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
                      work && blocks > 0, m, l);
   }
-  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
+  if (!ok && lane == 0) give_up(ctl, a.status);
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   if (warp == kWarpMma) {
     asm volatile("tcgen05.fence::after_thread_sync;");
+    drain_after_giving_up(ctl);
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
 }
@@ -698,7 +740,6 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
   constexpr uint32_t kO = 256;  // TMEM: score buffers at 0 and 128, O from 256
   constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kBlock >> 3) << 17) | (8u << 24);
   constexpr uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((uint32_t)(kD >> 3) << 17) | (8u << 24);
-  constexpr int kBarK = kBarSlot, kBarV = kBarSlot + 1;
   extern __shared__ uint8_t smem_raw[];
   wait_for_predecessor();
   let_successor_start();
@@ -725,6 +766,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     mbar_init(o_done, 1);
     mbar_init(o_last, 1);
     for (int i = 0; i < kMaskRing; ++i) mbar_init(smem_u32(&ctl->mask_full[i]), 4);
+    mbar_init(smem_u32(&ctl->drained), 1);
+    ctl->gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kWarpMma) {
@@ -745,7 +788,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     if (warp == kWarpMma) {
       bar_sync(kBarQ, 128 + 32);
       auto qk = [&](int j) {
-        bar_sync(kBarK, 128 + 32);
+        bar_sync(kBarWideK + (j & 1), 128 + 32);
         asm volatile("tcgen05.fence::after_thread_sync;");
         if (lane == 0) {
 #pragma unroll
@@ -760,8 +803,8 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
       if (blocks > 0) qk(0);
       for (int j = 0; j < blocks; ++j) {
         if (j + 1 < blocks) qk(j + 1);
-        bar_sync(kBarV, 128 + 32);
-        bar_sync(kBarP + (j & 1), 128 + 32);
+        bar_sync(kBarWideV + (j & 1), 128 + 32);
+        bar_sync(kBarWideP + (j & 3), 128 + 32);
         asm volatile("tcgen05.fence::after_thread_sync;");
         if (lane == 0) {
 #pragma unroll
@@ -798,15 +841,15 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     for (int j = 0; j < blocks; ++j) {
       const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
       if (j > 0 && ok)
-        ok = value ? mbar_wait(o_done, (j - 1) & 1)
-                   : mbar_wait(s_full[(j - 1) & 1], ((j - 1) >> 1) & 1);
+        ok = value ? warp_wait(o_done, (j - 1) & 1)
+                   : warp_wait(s_full[(j - 1) & 1], ((j - 1) >> 1) & 1);
       if (!value && lane == 0) {
         ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
         mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
       }
       store_row<kD>(r, value ? v_tile : k_tile, i);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      bar_arrive(value ? kBarV : kBarK, 128 + 32);
+      bar_tell(ok, (value ? kBarWideV : kBarWideK) + (j & 1), 128 + 32);
       pg = pg_next;
       pg_next = page_of(j + 2);
       fetch(r, j + 1, pg);
@@ -822,37 +865,38 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     float m = -INFINITY, l = 0.0f;
     uint32_t saw = 0;
     for (int j = 0; j < blocks; ++j) {
-      if (ok) ok = mbar_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      if (ok) ok = warp_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
       const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
-      if (ok) ok = mbar_wait(s_full[j & 1], (j >> 1) & 1);
+      if (ok) ok = warp_wait(s_full[j & 1], (j >> 1) & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
       // these scores were issued before the last P V, which O's rescaling must
       // wait for
       softmax_block<kD>(tmem + lanes + 128 * (j & 1), tmem + lanes + kO, masked, mask, w.scale,
                         j == 0, m, l, saw, [&] {
-                          if (ok) ok = mbar_wait(o_done, (j - 1) & 1);
+                          if (ok) ok = warp_wait(o_done, (j - 1) & 1);
                           asm volatile("tcgen05.fence::after_thread_sync;");
                         });
       // The next scores may be there before this P V is issued, so the softmax
-      // can be one block ahead of the MMA warp: two barriers in turn.  It cannot
-      // be two ahead, the scores after the next being issued behind this P V.
-      bar_arrive(kBarP + (j & 1), 128 + 32);
+      // can be one block ahead of the MMA warp.  It cannot be two ahead, the
+      // scores after the next being issued behind this P V.
+      bar_tell(ok, kBarWideP + (j & 3), 128 + 32);
     }
     // The last P V has a barrier of its own.  On o_done a warp would have to wait
     // for the one before it first, since a parity wait may not skip a phase, and
     // the last could complete before that wait looks: the phase that it waits for
     // would be gone, and the wait run out.
-    if (blocks > 0 && ok) ok = mbar_wait(o_last, 0);
+    if (blocks > 0 && ok) ok = warp_wait(o_last, 0);
     asm volatile("tcgen05.fence::after_thread_sync;");
     if (saw && l == 0.0f) l = 1.0f;
     store_result<kD>(p, w, r, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
   }
-  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
+  if (!ok && lane == 0) give_up(ctl, a.status);
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   if (warp == kWarpMma) {
     asm volatile("tcgen05.fence::after_thread_sync;");
+    drain_after_giving_up(ctl);
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }
 }

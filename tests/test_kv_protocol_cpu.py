@@ -2,7 +2,8 @@
 host: warps that meet on named barriers, wait for mbarriers with a limit, and
 issue matrix products that complete in order at any later time.  Whatever the
 order, every wait sees its phase and every product finds the operands that it
-should."""
+should; whichever waits give up, and even if no product ever completes, every
+warp reaches the end."""
 import random
 
 import pytest
@@ -79,7 +80,20 @@ class Machine:
                 state[w] = ("wait", step[1:])
 
 
-class Narrow:
+class Kernel:
+    apart = True  # as many barriers of a kind as arrivals may be outstanding, and one more
+    meet = True   # a warp that gave up waits at its barriers
+
+    def tell(self, ok, name, count):
+        return ("arrive" if ok or not self.meet else "sync", name, count)
+
+    def turn(self, name, j, turns, few):
+        """The barrier of block j's arrival: `turns` in turn, `few` if they were no more than the waits need
+        that do not give up."""
+        return name, j % (turns if self.apart else few)
+
+
+class Narrow(Kernel):
     """prompt_kernel: four slots (K, V, K, V), two halves.  Counts are in warps: 4 arrive, 1 takes part."""
 
     def __init__(self, m, blocks, two):
@@ -119,7 +133,7 @@ class Narrow:
             q.append(product)
         yield ("sync", "Q", 9)
         if self.blocks:
-            yield ("sync", ("slot", 0), 5)
+            yield ("sync", self.turn("K", 0, 4, 2), 5)
             qk(0, 0, 0)
             if self.two:
                 qk(1, 0, 0)
@@ -127,11 +141,11 @@ class Narrow:
                 q.append(lambda: m.mbar_arrive(("empty", 0)))
             for j in range(self.blocks):
                 v, k, more = (2 * j + 1) & 3, (2 * j + 2) & 3, j + 1 < self.blocks
-                yield ("sync", ("slot", v), 5)
+                yield ("sync", self.turn("V", j, 4, 2), 5)
                 if more:
-                    yield ("sync", ("slot", k), 5)
+                    yield ("sync", self.turn("K", j + 1, 4, 2), 5)
                 for half in range(2 if self.two else 1):
-                    yield ("sync", ("P", half), 5)
+                    yield ("sync", self.turn(("P", half), j, 2, 1), 5)
                     pv(half, v, j)
                     if more:
                         qk(half, k, j + 1)
@@ -152,7 +166,7 @@ class Narrow:
                 if side == "K":
                     self.m.mbar_arrive(("mask", j % 4))
                 self.slots[slot][warp] = (side, j)
-                yield ("arrive", ("slot", slot), 5)
+                yield self.tell(ok, self.turn(side, j, 4, 2), 5)
         yield ("sync", "end", 13)
 
     def softmax(self, half, warp):
@@ -167,7 +181,7 @@ class Narrow:
             if ok and not self.m.gave_up:
                 self.expect(self.scores[half], j, "S")
             self.weights[half][warp] = j
-            yield ("arrive", ("P", half), 5)
+            yield self.tell(ok, self.turn(("P", half), j, 2, 1), 5)
         if work and self.blocks and ok:
             ok = yield ("wait", ("s", half), self.blocks & 1)
             if ok and not self.m.gave_up:
@@ -175,7 +189,7 @@ class Narrow:
         yield ("sync", "end", 13)
 
 
-class Wide:
+class Wide(Kernel):
     """prompt_wide_kernel: one K and one V tile with four warps each, two score buffers."""
 
     together = False  # whether the last P V has the others' barrier
@@ -217,14 +231,14 @@ class Wide:
             q.append(lambda: m.mbar_arrive("o" if self.together or j + 1 < self.blocks else "last"))
         yield ("sync", "Q", 5)
         if self.blocks:
-            yield ("sync", "K", 5)
+            yield ("sync", self.turn("K", 0, 2, 1), 5)
             qk(0)
         for j in range(self.blocks):
             if j + 1 < self.blocks:
-                yield ("sync", "K", 5)
+                yield ("sync", self.turn("K", j + 1, 2, 1), 5)
                 qk(j + 1)
-            yield ("sync", "V", 5)
-            yield ("sync", ("P", j & 1), 5)
+            yield ("sync", self.turn("V", j, 2, 1), 5)
+            yield ("sync", self.turn("P", j, 4, 2), 5)
             pv(j)
         yield ("sync", "end", 13)
 
@@ -239,7 +253,7 @@ class Wide:
             if side == "K":
                 self.m.mbar_arrive(("mask", j % 4))
             self.tiles[side][warp] = j
-            yield ("arrive", side, 5)
+            yield self.tell(ok, self.turn(side, j, 2, 1), 5)
         yield ("sync", "end", 13)
 
     def softmax(self, warp):
@@ -255,7 +269,7 @@ class Wide:
             if j and ok and self.m.rng.random() < 0.5:  # a rescale of O
                 ok = yield ("wait", "o", (j - 1) & 1)
             self.weights[j & 1][warp] = j
-            yield ("arrive", ("P", j & 1), 5)
+            yield self.tell(ok, self.turn("P", j, 4, 2), 5)
         if self.together and self.blocks > 1 and ok:
             ok = yield ("wait", "o", (self.blocks - 2) & 1)
         if self.blocks and ok:
@@ -291,3 +305,28 @@ def test_one_barrier_for_all_products_would_miss_a_phase():
     """Why the last product has a barrier of its own: it may complete before a slow warp has looked for the one
     before it, whose phase is then over."""
     assert any(play(WideTogether, seed, seed % 11, 0, 0.0)[0].gave_up for seed in range(150))
+
+
+@pytest.mark.parametrize("kernel", [Narrow, Wide])
+@pytest.mark.parametrize("chance,stalled", [(0.002, False), (0.05, False), (0.5, False), (0.02, True), (1.0, True)])
+def test_every_warp_ends_whichever_waits_give_up(kernel, chance, stalled):
+    for seed in range(200):
+        m, _ = play(kernel, seed, seed % 13, seed % 2, chance, stalled)
+        assert all(arrived == 0 for arrived, _ in m.named.values()), seed
+
+
+def hangs(kernel):
+    for seed in range(200):
+        try:
+            play(kernel, seed, 12, 1, 0.02)
+        except Deadlock:
+            return True
+    return False
+
+
+@pytest.mark.parametrize("base", [Narrow, Wide])
+@pytest.mark.parametrize("apart,meet", [(False, False), (True, False), (False, True)])
+def test_either_rule_alone_would_hang(base, apart, meet):
+    """Why a warp that gave up waits at its barriers, and why they are used in turn: otherwise it can arrive
+    twice before its partner, which then waits for arrivals that were counted already."""
+    assert hangs(type("Planted", (base,), {"apart": apart, "meet": meet})) and not hangs(base)
