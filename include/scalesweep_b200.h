@@ -378,8 +378,8 @@ int ssw_nvfp4_kv_gather(const ssw_kv_cache* cache, int dtype, int64_t tokens,
  * q_heads], the natural log of the sum of exp(softmax_scale * q . K).
  * max_query_len and max_seq_len bound the batch's lengths from above; queries
  * and keys past them may be passed over.
- * status (may be null): an int set to 1 if a bounded device-side wait gave up
- * (the output is then undefined).
+ * status (may be null): an int set to 1 if a bounded device-side wait gave up;
+ * the rows that it left unfinished are then NaN.
  */
 typedef struct {
   const int32_t* block_table;

@@ -443,7 +443,11 @@ __device__ __forceinline__ void decode_tile(const Params& p) {
       phase ^= 1;
     }
   }
-  if (!ok && lane == 0 && a.status) atomicCAS(a.status, 0, 1);
+  if (!ok) {  // unfinished rows are NaN
+    if (lane == 0 && a.status) atomicCAS(a.status, 0, 1);
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) l[n][0] = l[n][1] = NAN;
+  }
 
   // ---- merge the warps through shared memory
 #pragma unroll

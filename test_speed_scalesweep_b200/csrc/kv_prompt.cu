@@ -24,7 +24,8 @@
 //
 // Every mbarrier wait is bounded; after one that gave up the roles keep their
 // barrier protocol, so no partner is left waiting (see bar_tell), MMAs in flight
-// are waited for, with a limit, and *status is set.
+// are waited for, with a limit, the rows that may be wrong become NaN and *status
+// is set.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -465,17 +466,20 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&v)[3
   __syncwarp();
 }
 
-// A wait has given up: what the caller, and the end of the CTA, go by.
-__device__ __forceinline__ void give_up(Control* ctl, int32_t* status) {
+// A wait has given up.  Said before the warp touches a tile that an MMA may still
+// read: who sees that MMA's result sees this as well, and makes its rows NaN.
+__device__ __forceinline__ void give_up(Control* ctl) {
   *reinterpret_cast<volatile uint32_t*>(&ctl->gave_up) = 1;
-  if (status) atomicCAS(status, 0, 1);
+}
+__device__ __forceinline__ bool gave_up(const Control* ctl) {
+  return *reinterpret_cast<const volatile uint32_t*>(&ctl->gave_up) != 0;
 }
 
 // The MMA warp, behind the last barrier: where a wait gave up, MMAs may still be
 // in flight, which read shared memory, write TMEM and arrive on barriers.  Waits
 // for them, with a limit as well, before TMEM is freed and the CTA ends.
 __device__ __forceinline__ void drain_after_giving_up(Control* ctl) {
-  if (*reinterpret_cast<const volatile uint32_t*>(&ctl->gave_up) == 0) return;
+  if (!gave_up(ctl)) return;
   if ((threadIdx.x & 31) == 0) mma_commit(smem_u32(&ctl->drained));
   mbar_wait(smem_u32(&ctl->drained), 0);
   __syncwarp();
@@ -583,6 +587,13 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
   asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
   bool ok = true;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (ok && !warp_wait(bar, parity)) {
+      ok = false;
+      give_up(ctl);
+      __syncwarp();
+    }
+  };
 
   if (warp >= kWarpMma) {
     fewer_registers<kRegsMma>();
@@ -664,7 +675,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       const int k_slot = (2 * j) & 3, v_slot = k_slot + 1;
       const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
       // slots are used every second block
-      if (j >= 2 && ok) ok = warp_wait(smem_u32(&ctl->empty[k_slot]), ((j >> 1) - 1) & 1);
+      if (j >= 2) wait(smem_u32(&ctl->empty[k_slot]), ((j >> 1) - 1) & 1);
       if (lane == 0) {
         ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
         mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
@@ -675,7 +686,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
       pg = pg_next;
       pg_next = page_of(j + 2);
       fetch(k, j + 1, pg, 0);
-      if (j >= 2 && ok) ok = warp_wait(smem_u32(&ctl->empty[v_slot]), ((j >> 1) - 1) & 1);
+      if (j >= 2) wait(smem_u32(&ctl->empty[v_slot]), ((j >> 1) - 1) & 1);
       store_row<kD>(v, ring + v_slot * S::kTile, i);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       bar_tell(ok, kBarSlot + ((2 * j + 1) & 7), 128 + 32);
@@ -696,23 +707,24 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     uint32_t saw = 0;
     const bool work = half == 0 || two;
     for (int j = 0; work && j < blocks; ++j) {
-      if (ok) ok = warp_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
       const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
-      if (ok) ok = warp_wait(smem_u32(&ctl->s_full[half]), j & 1);
+      wait(smem_u32(&ctl->s_full[half]), j & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
       // the P V before this S was issued before it, and has completed with it
       softmax_block<kD>(s_addr, o_addr, masked, mask, w.scale, j == 0, m, l, saw, [] {});
       bar_tell(ok, kBarP + 2 * half + (j & 1), 128 + 32);
     }
-    if (work && blocks > 0 && ok) ok = warp_wait(smem_u32(&ctl->s_full[half]), blocks & 1);
+    if (work && blocks > 0) wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
     if (saw && l == 0.0f) l = 1.0f;  // all its scores are -inf: see row_inverse
+    if (!ok || gave_up(ctl)) l = NAN;
     // this half's MMAs are done with its Q, which becomes the staging area
     store_result<kD>(p, w, half * 128 + r, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
                      work && blocks > 0, m, l);
   }
-  if (!ok && lane == 0) give_up(ctl, a.status);
+  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   if (warp == kWarpMma) {
@@ -782,6 +794,13 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
   asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
   bool ok = true;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (ok && !warp_wait(bar, parity)) {
+      ok = false;
+      give_up(ctl);
+      __syncwarp();
+    }
+  };
 
   if (warp >= kWarpMma) {
     fewer_registers<kRegsMma>();
@@ -840,9 +859,12 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     fetch(r, 0, pg);
     for (int j = 0; j < blocks; ++j) {
       const uint32_t there = __ballot_sync(0xFFFFFFFFu, pg >= 0);
-      if (j > 0 && ok)
-        ok = value ? warp_wait(o_done, (j - 1) & 1)
-                   : warp_wait(s_full[(j - 1) & 1], ((j - 1) >> 1) & 1);
+      if (j > 0) {
+        if (value)
+          wait(o_done, (j - 1) & 1);
+        else
+          wait(s_full[(j - 1) & 1], ((j - 1) >> 1) & 1);
+      }
       if (!value && lane == 0) {
         ctl->mask[j % kMaskRing][warp - kWarpDequant] = there;
         mbar_arrive(smem_u32(&ctl->mask_full[j % kMaskRing]));
@@ -865,16 +887,16 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     float m = -INFINITY, l = 0.0f;
     uint32_t saw = 0;
     for (int j = 0; j < blocks; ++j) {
-      if (ok) ok = warp_wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
+      wait(smem_u32(&ctl->mask_full[j % kMaskRing]), (j / kMaskRing) & 1);
       uint32_t mask[4];
       const bool masked = block_mask(ctl, j, c0 + j * kBlock, w, mask);
-      if (ok) ok = warp_wait(s_full[j & 1], (j >> 1) & 1);
+      wait(s_full[j & 1], (j >> 1) & 1);
       asm volatile("tcgen05.fence::after_thread_sync;");
       // these scores were issued before the last P V, which O's rescaling must
       // wait for
       softmax_block<kD>(tmem + lanes + 128 * (j & 1), tmem + lanes + kO, masked, mask, w.scale,
                         j == 0, m, l, saw, [&] {
-                          if (ok) ok = warp_wait(o_done, (j - 1) & 1);
+                          wait(o_done, (j - 1) & 1);
                           asm volatile("tcgen05.fence::after_thread_sync;");
                         });
       // The next scores may be there before this P V is issued, so the softmax
@@ -886,12 +908,13 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     // for the one before it first, since a parity wait may not skip a phase, and
     // the last could complete before that wait looks: the phase that it waits for
     // would be gone, and the wait run out.
-    if (blocks > 0 && ok) ok = warp_wait(o_last, 0);
+    if (blocks > 0) wait(o_last, 0);
     asm volatile("tcgen05.fence::after_thread_sync;");
     if (saw && l == 0.0f) l = 1.0f;
+    if (!ok || gave_up(ctl)) l = NAN;
     store_result<kD>(p, w, r, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
   }
-  if (!ok && lane == 0) give_up(ctl, a.status);
+  if (!ok && a.status && lane == 0) atomicCAS(a.status, 0, 1);
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   if (warp == kWarpMma) {

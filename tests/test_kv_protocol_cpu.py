@@ -3,7 +3,8 @@ host: warps that meet on named barriers, wait for mbarriers with a limit, and
 issue matrix products that complete in order at any later time.  Whatever the
 order, every wait sees its phase and every product finds the operands that it
 should; whichever waits give up, and even if no product ever completes, every
-warp reaches the end."""
+warp reaches the end, and a row whose products did not all find what they
+should is marked."""
 import random
 
 import pytest
@@ -22,6 +23,9 @@ class Machine:
     def __init__(self, rng, give_up, stalled):
         self.rng, self.give_up, self.stalled = rng, give_up, stalled
         self.named, self.mbar, self.queue, self.gave_up = {}, {}, [], False
+        self.flag = False  # what the warps see of it
+
+    late = False  # whether a warp that gave up says so at its end only
 
     def init(self, name, count):
         self.mbar[name] = [0, count, count]  # phases completed, arrivals missing, count
@@ -60,9 +64,11 @@ class Machine:
                 continue
             if value is False:
                 self.gave_up = True
+                self.flag = self.flag or not self.late
             try:
                 step = w.send(value)
             except StopIteration:
+                self.flag = self.flag or self.gave_up
                 del state[w]
                 continue
             if step[0] in ("arrive", "sync"):
@@ -87,6 +93,14 @@ class Kernel:
     def tell(self, ok, name, count):
         return ("arrive" if ok or not self.meet else "sync", name, count)
 
+    def spoil(self, half, all_rows, rows=(False,) * 4):
+        self.spoiled |= {(half, i) for i in range(4) if all_rows or rows[i]}
+
+    def finish(self, ok, half, warp, complete):
+        """A softmax warp is about to store its rows."""
+        if ok and not self.m.flag and (not complete or (half, warp) in self.spoiled):
+            self.unmarked.append((half, warp))
+
     def turn(self, name, j, turns, few):
         """The barrier of block j's arrival: `turns` in turn, `few` if they were no more than the waits need
         that do not give up."""
@@ -106,6 +120,7 @@ class Narrow(Kernel):
         self.slots = [[None] * 4 for _ in range(4)]  # what each dequantizing warp last stored
         self.scores, self.weights = [None, None], [[None] * 4 for _ in range(2)]
         self.done, self.wrong = [], []
+        self.spoiled, self.unmarked = set(), []  # (half, warp) whose rows a product took from elsewhere; and not marked
 
     def warps(self):
         out = [self.mma()] + [self.dequant(i) for i in range(4)]
@@ -121,6 +136,7 @@ class Narrow(Kernel):
         def qk(half, slot, j):
             def product():
                 self.expect(self.slots[slot], [("K", j)] * 4, "K")
+                self.spoil(half, self.slots[slot] != [("K", j)] * 4)
                 self.scores[half] = j
             q.append(product)
             q.append(lambda: m.mbar_arrive(("s", half)))
@@ -129,6 +145,7 @@ class Narrow(Kernel):
             def product():
                 self.expect(self.slots[slot], [("V", j)] * 4, "V")
                 self.expect(self.weights[half], [j] * 4, "P")
+                self.spoil(half, self.slots[slot] != [("V", j)] * 4, [x != j for x in self.weights[half]])
                 self.done.append((half, j))
             q.append(product)
         yield ("sync", "Q", 9)
@@ -186,6 +203,8 @@ class Narrow(Kernel):
             ok = yield ("wait", ("s", half), self.blocks & 1)
             if ok and not self.m.gave_up:
                 self.expect((half, self.blocks - 1) in self.done, True, "O")
+        if work and self.blocks:
+            self.finish(ok, half, warp, (half, self.blocks - 1) in self.done)
         yield ("sync", "end", 13)
 
 
@@ -205,6 +224,7 @@ class Wide(Kernel):
         self.tiles = {"K": [None] * 4, "V": [None] * 4}
         self.scores, self.weights = [None, None], [[None] * 4 for _ in range(2)]
         self.done, self.wrong = [], []
+        self.spoiled, self.unmarked = set(), []
 
     expect = Narrow.expect
 
@@ -218,6 +238,7 @@ class Wide(Kernel):
         def qk(j):
             def product():
                 self.expect(self.tiles["K"], [j] * 4, "K")
+                self.spoil(0, self.tiles["K"] != [j] * 4)
                 self.scores[j & 1] = j
             q.append(product)
             q.append(lambda: m.mbar_arrive(("s", j & 1)))
@@ -226,6 +247,7 @@ class Wide(Kernel):
             def product():
                 self.expect(self.tiles["V"], [j] * 4, "V")
                 self.expect(self.weights[j & 1], [j] * 4, "P")
+                self.spoil(0, self.tiles["V"] != [j] * 4, [x != j for x in self.weights[j & 1]])
                 self.done.append(j)
             q.append(product)
             q.append(lambda: m.mbar_arrive("o" if self.together or j + 1 < self.blocks else "last"))
@@ -276,12 +298,14 @@ class Wide(Kernel):
             ok = yield ("wait", "o", (self.blocks - 1) & 1) if self.together else ("wait", "last", 0)
             if ok and not self.m.gave_up:
                 self.expect(self.done[-1:], [self.blocks - 1], "O")
+        if self.blocks:
+            self.finish(ok, 0, warp, self.done[-1:] == [self.blocks - 1])
         yield ("sync", "end", 13)
 
 
-def play(kernel, seed, blocks, two, chance, stalled=False):
+def play(kernel, seed, blocks, two, chance, stalled=False, machine=Machine):
     rng = random.Random(seed)
-    m = Machine(rng, lambda r: r.random() < chance, stalled)
+    m = machine(rng, lambda r: r.random() < chance, stalled)
     k = kernel(m, blocks, two)
     m.run(k.warps())
     return m, k
@@ -311,8 +335,9 @@ def test_one_barrier_for_all_products_would_miss_a_phase():
 @pytest.mark.parametrize("chance,stalled", [(0.002, False), (0.05, False), (0.5, False), (0.02, True), (1.0, True)])
 def test_every_warp_ends_whichever_waits_give_up(kernel, chance, stalled):
     for seed in range(200):
-        m, _ = play(kernel, seed, seed % 13, seed % 2, chance, stalled)
+        m, k = play(kernel, seed, seed % 13, seed % 2, chance, stalled)
         assert all(arrived == 0 for arrived, _ in m.named.values()), seed
+        assert not k.unmarked, seed
 
 
 def hangs(kernel):
@@ -330,3 +355,13 @@ def test_either_rule_alone_would_hang(base, apart, meet):
     """Why a warp that gave up waits at its barriers, and why they are used in turn: otherwise it can arrive
     twice before its partner, which then waits for arrivals that were counted already."""
     assert hangs(type("Planted", (base,), {"apart": apart, "meet": meet})) and not hangs(base)
+
+
+class LateMachine(Machine):
+    late = True
+
+
+@pytest.mark.parametrize("kernel", [Narrow, Wide])
+def test_said_at_the_end_only_rows_would_stay_unmarked(kernel):
+    """Why a warp says that it gave up before it goes on: another may store rows made of what it wrote."""
+    assert any(play(kernel, seed, 12, 1, 0.02, machine=LateMachine)[1].unmarked for seed in range(400))
