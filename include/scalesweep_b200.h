@@ -452,7 +452,7 @@ int ssw_kv_pages_fork(const ssw_kv_pages* tables, const ssw_kv_pool* pool, int64
                       const int32_t* parents, const int32_t* children, void* workspace,
                       int64_t workspace_bytes, void* stream);
 /* The sequences become empty; pages that nothing refers to any more are free.
- * A sequence named twice is freed once; one out of range is passed over. */
+ * A sequence named twice is freed once. */
 int ssw_kv_pages_free(const ssw_kv_pages* tables, int64_t n, const int32_t* seqs, void* stream);
 /* new_tokens[i] tokens more for sequence seqs[i]; slot_mapping [total_tokens]
  * gets their slots, sequence by sequence (-1 where the call was not served).

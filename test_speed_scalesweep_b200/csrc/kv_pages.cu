@@ -241,16 +241,21 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply(const PagesArgs a, co
   }
 }
 
-// ---- free: one CTA per sequence; a sequence named twice is freed once
+// ---- free: one CTA per sequence; a sequence named twice is freed once.  Every CTA
+// looks at all the indices first (at most a few reads per thread), so that with
+// one out of range none frees anything.
 __global__ void __launch_bounds__(kCopyThreads) free_kernel(const PagesArgs a) {
   wait_for_predecessor();
   let_successor_start();
   __shared__ int old;
-  const int s = a.seqs[blockIdx.x];
-  if ((uint32_t)s >= (uint32_t)a.max_seqs) {
-    report(a.status, kPagesBadIndex);
+  int bad = 0;
+  for (int i = threadIdx.x; i < a.n; i += kCopyThreads)
+    bad |= (uint32_t)a.seqs[i] >= (uint32_t)a.max_seqs;
+  if (__syncthreads_or(bad)) {
+    if (blockIdx.x == 0) report(a.status, kPagesBadIndex);
     return;
   }
+  const int s = a.seqs[blockIdx.x];
   if (threadIdx.x == 0) old = atomicExch(&a.seq_lens[s], 0);
   __syncthreads();
   const int page_mask = (1 << a.page_shift) - 1;

@@ -60,8 +60,9 @@ class NVFP4KVPages:
         self._kv.pages_fork(self._pages, parents, children)
 
     def free(self, seqs: torch.Tensor) -> None:
-        """Empty the sequences ``seqs`` (int32).  Pages that no other sequence
-        shares become free; their bytes stay until they are taken again."""
+        """Empty the sequences ``seqs`` (int32; one named twice is freed once).
+        Pages that no other sequence shares become free; their bytes stay until
+        they are taken again."""
         self._kv.pages_free(self._pages, seqs)
 
     def compact(self) -> None:
