@@ -414,8 +414,10 @@ int ssw_nvfp4_paged_attention(const ssw_kv_cache* cache, const ssw_kv_attention*
  * to it; pages are taken lowest first, in the order of the requests.  A call
  * that cannot be served as a whole changes nothing, and status (may be null)
  * becomes, unless it is nonzero already: 1 not enough free pages, 2 a sequence
- * out of range, named twice, or (fork) a child that is not empty, 3 a sequence
- * longer than its row.  A pool is the cache's bytes over all layers.
+ * out of range, named twice (free takes it once), (fork) a child that is not
+ * empty or (extend) new tokens that are negative or do not add up to
+ * total_tokens, 3 a sequence longer than its row.  A pool is the cache's bytes
+ * over all layers.
  */
 typedef struct {
   int32_t* refcount;    /* [num_pages] */

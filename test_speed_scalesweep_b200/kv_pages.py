@@ -10,7 +10,8 @@ import torch
 from . import _lib
 
 _STATUS = {1: "not enough free pages",
-           2: "a sequence index is out of range, named twice, or a child that is not empty",
+           2: "a sequence index is out of range or named twice, a child is not empty, or new tokens "
+              "are negative or do not add up to their total",
            3: "a sequence is longer than its row of the block table"}
 
 
@@ -26,7 +27,8 @@ class NVFP4KVPages:
     Pages are taken lowest first, in the order of the requests.  A request that
     cannot be served changes nothing and leaves a code in ``status`` (int32
     ``[1]``), which :meth:`check` reads.  A part-filled page must belong to one
-    sequence alone; :meth:`fork` keeps it so."""
+    sequence alone; :meth:`fork` keeps it so.  :meth:`copy` is no request on the
+    tables and leaves no code."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, block_table: torch.Tensor,
                  seq_lens: torch.Tensor, refcount: torch.Tensor,
@@ -72,7 +74,8 @@ class NVFP4KVPages:
 
     def copy(self, source: torch.Tensor, target: torch.Tensor) -> None:
         """Copy page ``source[i]`` to ``target[i]`` (int32) in every layer.
-        Targets are distinct, and none is a source; the tables do not change."""
+        Targets are distinct, and none is a source; a pair with a page outside
+        the cache is passed over.  The tables do not change."""
         self._kv.pages_copy(self._pages, source, target)
 
     def check(self) -> None:

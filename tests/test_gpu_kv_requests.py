@@ -45,3 +45,12 @@ def test_free_in_a_graph(pages):  # noqa: F811
         m.compare(t)
         t.free(i32([0, 1, 2, 3]))
         m.free([0, 1, 2, 3])
+
+
+@pytest.mark.parametrize("more,total", [([3], 5), ([3], 2), ([-1], 0)])
+def test_the_message_names_a_wrong_total(pages, more, total):  # noqa: F811
+    t, m = make(pages, 8, 4, 3, layers=1), Model(8, 4, 3, 16)
+    assert t.extend(i32([2]), i32(more), total).tolist() == [-1] * total
+    with pytest.raises(RuntimeError, match="add up"):
+        t.check()
+    m.compare(t)
