@@ -14,6 +14,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -150,6 +151,16 @@ ssw_kv_heads heads_of(const at::Tensor& t, const char* name, int64_t tokens, int
   return {t.data_ptr(), st, sh};
 }
 
+// These calls bypass autograd, so a gradient that is asked for would be lost
+// without a word.
+void check_no_gradient(const at::Tensor& t, const char* name) {
+  if (c10::GradMode::is_enabled() && t.requires_grad())
+    bad("%s requires a gradient, which this operator does not have: call it under torch.no_grad()",
+        name);
+  if (at::isFloatingType(t.scalar_type()) && t._fw_grad(0).defined())
+    bad("%s carries a forward-mode gradient, which this operator does not have", name);
+}
+
 // An output whose elements share memory would be written in no order.
 void check_distinct(const at::Tensor& t, const char* name) {
   for (int64_t i = 0; i < t.dim(); ++i)
@@ -209,6 +220,11 @@ PyObject* write(PyObject*, PyObject* const* x, Py_ssize_t n) {
                      &scales = tensor(x[8], "scales");
     const ssw_kv_cache cache = cache_of(codes, scales, mult);
     const c10::Device dev = codes.device();
+    check_no_gradient(query, "query");
+    check_no_gradient(key, "key");
+    check_no_gradient(value, "value");
+    check_no_gradient(table, "cos_sin_cache");
+    check_no_gradient(mult, "kv_input_scale");
     if (query.dim() != 3)
       bad("query must be [T, heads, head_size], got shape %s", shape_of(query).c_str());
     const int64_t tokens = query.size(0), hq = query.size(1), d = query.size(2);
@@ -231,6 +247,7 @@ PyObject* write(PyObject*, PyObject* const* x, Py_ssize_t n) {
         x[10] == Py_None ? empty({tokens, hq, d}, type, dev) : tensor(x[10], "query_out");
     const ssw_kv_heads o = heads_of(out, "query_out", tokens, hq, d, type, dev);
     check_distinct(out, "query_out");
+    check_no_gradient(out, "query_out");
     check_status(ssw_rotary_scalesweep_mse_nvfp4_kv_write(
         &cache, dtype, tokens, (int)hq, &q, &k, &v, &o, static_cast<const int64_t*>(pos),
         static_cast<const float*>(table.data_ptr()), table.size(0), (int)table.size(1),
@@ -254,6 +271,7 @@ PyObject* gather(PyObject*, PyObject* const* x, Py_ssize_t n) {
     const int dtype = dtype_code(type);
     const ssw_kv_cache cache = cache_of(codes, scales, mult);
     const c10::Device dev = codes.device();
+    check_no_gradient(mult, "kv_input_scale");
     const int64_t tokens = slots.numel();
     const void* slot = vector_of(slots, "slot_mapping", at::kLong, tokens, dev);
     const c10::cuda::CUDAGuard guard(dev);
@@ -282,6 +300,8 @@ PyObject* attend(PyObject*, PyObject* const* x, Py_ssize_t n) {
                      &start = tensor(x[6], "query_start");
     const ssw_kv_cache cache = cache_of(codes, scales, mult);
     const c10::Device dev = codes.device();
+    check_no_gradient(query, "query");
+    check_no_gradient(mult, "kv_input_scale");
     if (query.dim() != 3)
       bad("query must be [T, heads, head_size], got shape %s", shape_of(query).c_str());
     const int64_t tokens = query.size(0), hq = query.size(1), d = query.size(2);
@@ -340,6 +360,7 @@ PyObject* attend(PyObject*, PyObject* const* x, Py_ssize_t n) {
         x[12] == Py_None ? empty({tokens, hq, d}, type, dev) : tensor(x[12], "out");
     const ssw_kv_heads o = heads_of(out, "out", tokens, hq, d, type, dev);
     check_distinct(out, "out");
+    check_no_gradient(out, "out");
     at::Tensor lse, workspace;
     if (want_lse) {
       lse = empty({tokens, hq}, at::kFloat, dev);

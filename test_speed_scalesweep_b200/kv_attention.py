@@ -39,7 +39,10 @@ def nvfp4_paged_attention(query: torch.Tensor, codes: torch.Tensor, scales: torc
     as they were; without ``out`` a new tensor, those rows undefined), with
     ``return_lse`` also the float32 [T, Hq] natural log-sum-exp of the scores.
     ``status``: optional int32 device tensor, set to 1 if a bounded wait inside
-    the kernel gave up; the rows that it left unfinished are NaN."""
+    the kernel gave up; the rows that it left unfinished are NaN.
+
+    There is no backward pass: a query that requires a gradient is refused outside
+    ``torch.no_grad()``."""
     return _lib.kv_binding().attend(query, codes, scales, kv_input_scale, block_table, seq_lens,
                                     query_start, max_query_len, max_seq_len, softmax_scale, causal,
                                     window, out, return_lse, status)

@@ -119,7 +119,8 @@ def rotary_scalesweep_mse_nvfp4_kv_write(query: torch.Tensor, key: torch.Tensor,
     in place, any other overlaps no input), else a new contiguous tensor.
     ``key`` and ``value`` are only read.  Rows whose slot is negative or past the last page are padding: not
     stored.  Slots must be distinct.  A position outside the table gives NaN in
-    the query, and that token is not stored."""
+    the query, and that token is not stored.  There is no backward pass: inputs
+    that require a gradient are refused outside ``torch.no_grad()``."""
     return _lib.kv_binding().write(query, key, value, positions, cos_sin_cache, slot_mapping,
                                    kv_input_scale, codes, scales, is_neox, query_out)
 
