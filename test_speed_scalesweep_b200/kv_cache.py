@@ -30,6 +30,19 @@ from . import _lib
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_SIZES = (64, 128, 256)
 
+# What a rope_scaling may hold, by rope_type, and what any may: names, and keys
+# that do not change the frequencies of a given rotary_dim.
+_SCALING_KEYS = {
+    "default": (), "linear": ("factor",),
+    "llama3": ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings"),
+    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor",
+             "mscale", "mscale_all_dim", "truncate")}
+_SCALING_REQUIRED = {
+    "default": (), "linear": ("factor",), "llama3": _SCALING_KEYS["llama3"],
+    "yarn": ("factor", "original_max_position_embeddings")}
+_SCALING_ANY = ("rope_type", "type", "rope_theta", "partial_rotary_factor", "max_position_embeddings",
+                "original_max_position_embeddings", "mrope_section", "mrope_interleaved")
+
 
 def alloc_kv_cache(num_pages: int, page_size: int, kv_heads: int, head_size: int,
                    device: torch.device | str = "cuda", num_layers: int | None = None):
@@ -59,7 +72,8 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
     ``original_max_position_embeddings``) or ``yarn`` (``factor``,
     ``original_max_position_embeddings``, optionally ``beta_fast``,
     ``beta_slow`` and ``attention_factor``, which multiplies both tables).
-    Keys that would change the frequencies in another way are refused.
+    Other keys are refused, and so is a ``rope_theta`` that is not ``base``;
+    a key that is None counts as absent.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
@@ -68,7 +82,18 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
     i = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
     freq = float(base) ** (-i / rotary_dim)
     mult = 1.0
-    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    scaling = {k: v for k, v in (scaling or {}).items() if v is not None}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"unsupported rope_type {kind!r}")
+    missing = [k for k in _SCALING_REQUIRED[kind] if k not in scaling]
+    if missing:
+        raise ValueError(f"{kind}: scaling needs {', '.join(missing)}")
+    unknown = sorted(set(scaling) - set(_SCALING_KEYS[kind]) - set(_SCALING_ANY))
+    if unknown:
+        raise ValueError(f"{kind}: unsupported keys {', '.join(unknown)}")
+    if "rope_theta" in scaling and float(scaling["rope_theta"]) != float(base):
+        raise ValueError(f"scaling has rope_theta {scaling['rope_theta']}, but base is {base}")
     if kind == "linear":
         freq = freq / float(scaling["factor"])
     elif kind == "llama3":
@@ -93,8 +118,6 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
         freq = freq / factor * ramp + freq * (1 - ramp)
         mult = scaling.get("attention_factor")
         mult = 0.1 * math.log(factor) + 1.0 if mult is None else float(mult)
-    elif kind != "default":
-        raise ValueError(f"unsupported rope_type {kind!r}")
     angle = torch.arange(max_position, dtype=torch.float64, device=device)[:, None] * freq
     return torch.cat([angle.cos() * mult, angle.sin() * mult], dim=-1).float()
 
