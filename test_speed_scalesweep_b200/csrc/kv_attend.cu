@@ -721,9 +721,9 @@ Plan plan_of(const AttendArgs& a, int device_sms) {
   const int group = a.q_heads / a.cache.kv_heads;
   const int64_t rows = (int64_t)a.max_query_len * group;
   // Rows up to which decode_kernel is the faster one (32 sequences of 8192 keys, 8
-  // kv heads, 32 rows: heads of 64 in one tile 148 us, 231 on the tensor cores'
-  // own memory; heads of 128 in two tiles of 16 239 and 271; heads of 256 so 422
-  // and 372).
+  // kv heads, 32 rows: heads of 64 in one tile 142 us, 234 on the tensor cores'
+  // own memory; heads of 128 in two tiles of 16 226 and 274; heads of 256 so 422
+  // and 371).
   const int most = a.cache.head_size == 256 ? 16 : 32;
   const int64_t sms = device_sms;
   Plan pl = {};

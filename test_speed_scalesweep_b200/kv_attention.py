@@ -2,8 +2,14 @@
 of prompts and batches that mix both, in one call.
 
 Keys and values stay in 4 bits until they are in registers or shared memory;
-a scale times a code has 6 significant bits, so 16-bit floats hold it exactly
-and the only roundings are those of the softmax weights and of the result."""
+a scale times a code has 6 significant bits, so 16-bit floats (f16) hold it
+exactly.  What is rounded to 16 bits: a bf16 query to f16, the softmax weights
+(f16, in units that keep full precision down to 2^-24 of the largest) and the
+result.  f16 holds bf16 values from 2^-17 to 2^16 exactly.  Single tokens and
+short queries are scaled by a power of two per row first, so that only elements
+below 2^-17 of the row's largest are rounded; rows of longer queries only where
+their largest lies outside 2^-6 .. 2^15, so that otherwise elements below 2^-17
+are rounded, by at most 2^-19 of the largest.  Sums are float32."""
 from __future__ import annotations
 
 import torch
@@ -33,7 +39,9 @@ def nvfp4_paged_attention(query: torch.Tensor, codes: torch.Tensor, scales: torc
     queries being the last of its keys.  ``window``: only those at most
     ``window`` positions before it.  ``softmax_scale`` defaults to D ** -0.5.
     A row that sees no key gives zeros (log-sum-exp -inf); NaN or an infinity in
-    a query row that sees one gives NaN, in that row alone.
+    a query row that sees one gives NaN, in that row alone.  (The cache's scales
+    are finite, as the write leaves them: a foreign NaN scale of a key that some
+    query sees makes NaN of rows that share work with that query's.)
 
     Returns ``out`` [T, Hq, D] of the query's type (rows of no sequence are left
     as they were; without ``out`` a new tensor, those rows undefined), with
