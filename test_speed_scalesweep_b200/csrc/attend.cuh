@@ -159,17 +159,22 @@ __device__ __forceinline__ int used_splits(const Params& p, const Tile& t) {
   return min(max(1, (n + p.chunk - 1) / p.chunk), p.splits);
 }
 
-// How a row is finished.  Its sum l of weights says whether it saw a key: a key
-// that it sees adds 2^kShift or more to l by the time the maximum m is final, a
-// masked one exactly 0.  A row whose scores so far are all -inf has m = -inf and a
-// positive l (in decode_kernel the keys that it saw), so that it is told from a
-// row that saw none; that l is dropped (times 2^-inf) when a larger score comes.
-// A NaN score makes l NaN and leaves m alone.
+// How a row is finished.  It saw no key where its maximum m is -inf and its sum l
+// of weights 0, a masked key's weight.  A NaN score makes l NaN and leaves m alone.
+// A row whose scores so far are all -inf has m = -inf and a positive l (in
+// decode_kernel the keys that it saw), which is dropped (times 2^-inf) when a
+// larger score comes.
 
 // 1 / (l * multiplier); 0 for a row that saw no key, whose result is zero; NaN
-// where every score is -inf, the weights being 0 / 0.
+// where every score is -inf, the weights being 0 / 0.  NaN, too, from |m| = 2^28
+// on: m and m - kShift are each off by up to half a step of m, so the largest
+// weight is 2^kShift times 2^-32 to 2^32 there, and below 2^-24 times that it
+// would be lost to f16, silently.  (From 2^23 on it may pass f16's largest, and the
+// result is infinite.)
 __device__ __forceinline__ float row_inverse(float m, float l, float inv_mult) {
-  return l == 0.0f ? 0.0f : m == -INFINITY ? NAN : inv_mult / l;
+  return fabsf(m) < 0x1p28f            ? inv_mult / l
+         : m == -INFINITY && l == 0.0f ? 0.0f
+                                       : NAN;
 }
 // Natural log-sum-exp: -inf for a row that saw no key (-inf + log2 0).
 __device__ __forceinline__ float row_lse(float m, float l) { return (m - kShift + log2f(l)) * kLn2; }

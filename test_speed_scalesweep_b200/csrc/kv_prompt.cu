@@ -493,7 +493,7 @@ __device__ __forceinline__ void store_result(const Params& p, const Row& w, int 
                                              uint32_t o_addr, uint32_t stage, bool any, float m,
                                              float l) {
   const AttendArgs& a = p.a;
-  const bool seen = any && l != 0.0f;  // a row that saw no key is zero
+  const bool seen = any && !(m == -INFINITY && l == 0.0f);  // a row that saw no key is zero
   if (p.splits == 1) {
     const float inv = row_inverse(m, l, 1.0f / a.cache.multiplier[1]);
 #pragma unroll 1
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_kernel(const Params p) {
     }
     if (work && blocks > 0) wait(smem_u32(&ctl->s_full[half]), blocks & 1);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    if (saw && l == 0.0f) l = 1.0f;  // all its scores are -inf: see row_inverse
+    if (saw && m == -INFINITY && l == 0.0f) l = 1.0f;  // all its scores are -inf: see row_inverse
     if (!ok || gave_up(ctl)) l = NAN;
     // this half's MMAs are done with its Q, which becomes the staging area
     store_result<kD>(p, w, half * 128 + r, o_addr, q_tile + half * S::kTile + (warp & 3) * 4096,
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(kPThreads, 1) prompt_wide_kernel(const Params 
     // would be gone, and the wait run out.
     if (blocks > 0) wait(o_last, 0);
     asm volatile("tcgen05.fence::after_thread_sync;");
-    if (saw && l == 0.0f) l = 1.0f;
+    if (saw && m == -INFINITY && l == 0.0f) l = 1.0f;
     if (!ok || gave_up(ctl)) l = NAN;
     store_result<kD>(p, w, r, tmem + lanes + kO, q_tile + warp * 4096, blocks > 0, m, l);
   }

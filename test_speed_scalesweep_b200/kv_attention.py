@@ -39,7 +39,9 @@ def nvfp4_paged_attention(query: torch.Tensor, codes: torch.Tensor, scales: torc
     queries being the last of its keys.  ``window``: only those at most
     ``window`` positions before it.  ``softmax_scale`` defaults to D ** -0.5.
     A row that sees no key gives zeros (log-sum-exp -inf); NaN or an infinity in
-    a query row that sees one gives NaN, in that row alone.  (The cache's scales
+    a query row that sees one gives NaN, in that row alone.  Scores are float32
+    in units of log 2: a row whose largest lies past 2^23 may not be finite, past
+    2^28 it is NaN.  (The cache's scales
     are finite, as the write leaves them: a foreign NaN scale of a key that some
     query sees makes NaN of rows that share work with that query's.)
 

@@ -94,3 +94,21 @@ def test_a_position_outside_the_table_stays_marked(attn, lens):  # noqa: F811
     b.q = kv_cache.rotary_scalesweep_mse_nvfp4_kv_write(b.q, kv, kv, pos, table, nowhere, b.mult, b.codes, b.scales)
     out = b.call(attn)
     assert bool(out[-1].isnan().all()) and bool(out[:-1].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("scale", [30.0, 1e6, 1e30])
+@pytest.mark.parametrize("cut", CUTS)
+def test_scores_past_what_float32_resolves_are_not_taken_for_no_key(attn, cut, scale, dtype):  # noqa: F811
+    """Where neighbouring float32 scores lie further apart than softmax can weigh, a row may be NaN, but not zero:
+    it saw keys, and their values are not 0."""
+    b = Batch(*CUTS[cut], dtype, seed=14, spread=3e3)
+    b.mult.fill_(1.0)
+    b.codes[:, 1] = (b.codes[:, 1] & 0x77) | 0x11  # values of at least 0.5 times their scale
+    out = b.call(attn, softmax_scale=scale)
+    at = 0
+    for n, m in b.lens:
+        for i in range(m):
+            none = n - m + i < 0 or n == 0
+            assert bool((out[at + i] == 0).all()) if none else not bool((out[at + i] == 0).any()), (at + i, none)
+        at += m
