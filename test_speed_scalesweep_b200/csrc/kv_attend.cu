@@ -543,10 +543,11 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const Params p, int tile
   const int head = blockIdx.z, seq = blockIdx.x / p.tiles;
   const int r = blockIdx.y * (kWarps / kPerRow) + (threadIdx.x >> 5) / kPerRow;
   // Everything that does not read the other grid's results comes before the
-  // wait (behind it, 64 sequences took 95 us against 94): the other grid has
-  // let this one start after waiting for what wrote the inputs, and writes none
-  // of them itself; the fence keeps these loads from lines that the SM's cache
-  // had before.  CTAs without a row wait too, so that this grid does not end first.
+  // wait (behind it, 64 sequences took 95 us against 94): the other grid or,
+  // beside prompts, the one before it let this one start after waiting for what
+  // wrote the inputs, and writes none of them; the fence keeps these loads from
+  // lines that the SM's cache had before.  CTAs without a row wait too, so that
+  // this grid does not end first.
   __threadfence();
   Tile tile;
   if (!tile_of(p, seq, blockIdx.x % p.tiles, tile_rows, tile) || r >= tile.rows) {
